@@ -214,6 +214,87 @@ int int4_linear_pack_i32(const int* src_d, void* dst_d, int rows, int cols, void
 int int4_linear_pack_i8(const signed char* src_d, void* dst_d, int rows, int cols, void* stream);
 int int4_linear_unpack_i32(const void* src_d, int* dst_d, int rows, int cols, void* stream);
 
+/*
+ * ------------------------------------------------------------------------------------------------
+ * Microscaled 4-bit floating point.  The reference has integers only; these operators are the same
+ * linear layer on the 4-bit format that the GPU's tensor cores multiply directly.
+ *
+ * A matrix is `rows` x `k` e2m1 codes (0, 1/2, 1, 3/2, 2, 3, 4, 6; bit 3 = sign), packed as the s4
+ * operands are (two per byte, low nibble = even index, row pitch k / 2 bytes), with one scale byte per
+ * block of a row:
+ *   INT4L_FP4_MX  blocks of 32; byte b stands for 2^(b - 127), 0xFF for NaN
+ *   INT4L_FP4_NV  blocks of 16; the byte is an e4m3 value; besides, one float for the whole matrix
+ *                 (tensor_scale, a device pointer; NULL = 1)
+ * Scale bytes lie in tiles of 128 rows x 4 scales, 512 bytes each: scale (r, j) of a tile at byte
+ * (r % 32) * 16 + (r / 32) * 4 + j.  The tiles of 128 rows follow one another along k, the groups of
+ * 128 rows along the rows; rows are padded to 128 and scales to 4, and the padding along k must not be
+ * NaN (int4_linear_fp4_quantize_async writes 0 everywhere in it).
+ *
+ * k % 32 == 0; codes and scales are 16-byte aligned device pointers.  Everything is asynchronous on
+ * `stream` and returns a status code.  An output may not overlap an input.
+ */
+#define INT4L_FP4_MX 0
+#define INT4L_FP4_NV 1
+
+#define INT4L_TYPE_BF16 0
+#define INT4L_TYPE_F16  1
+#define INT4L_TYPE_F32  2
+
+#define INT4L_ACT_SILU      0  /* g / (1 + exp(-g))                                  */
+#define INT4L_ACT_GELU      1  /* g times the normal distribution function of g      */
+#define INT4L_ACT_GELU_TANH 2  /* its tanh form                                      */
+
+typedef struct int4_linear_fp4_matrix {
+    const void* codes;
+    const void* scales;
+    const float* tensor_scale;  /* INT4L_FP4_NV only */
+    int rows, k, format;
+} int4_linear_fp4_matrix;
+
+/* Bytes of the scales of a matrix, or -INT4L_ERR_INVALID_ARG. */
+long long int4_linear_fp4_scale_bytes(int rows, int k, int format);
+
+/* Quantises a rows x k matrix of floats (src_type: INT4L_TYPE_*, row pitch src_pitch elements) into
+ * dst->codes and dst->scales, which are written in full, padding of the scales included.
+ *   MX  scale 2^e with e = floor(log2 amax) - 2, at least 2^-127 (amax: largest magnitude of the block)
+ *   NV  values are first multiplied by 1 / *tensor_scale, rounded to fp32 (a tensor_scale of 0 counts as
+ *       one of infinity: all codes 0); scale = amax / 6 to the nearest e4m3 value, at most 448
+ * codes = value / scale to the nearest e2m1 value, ties to the even code, at most 6 in magnitude; 0
+ * where the scale is 0.  A block with a NaN or an infinity gets the scale NaN. */
+int int4_linear_fp4_quantize_async(const void* src_d, int src_type, long long src_pitch,
+                                   const int4_linear_fp4_matrix* dst, void* stream);
+
+/* The values a matrix stands for, rows x k, contiguous, 16-byte aligned, rounded once to dst_type. */
+int int4_linear_fp4_dequantize_async(const int4_linear_fp4_matrix* src, void* dst_d, int dst_type, void* stream);
+
+/* y[m x n] = x[m x k] w[n x k]^T + bias, accumulated in fp32, rounded once to y_type (BF16 or F16).
+ * x and w have one format; bias_d is n floats or NULL. */
+int int4_linear_fp4_launch_async(const int4_linear_fp4_matrix* x, const int4_linear_fp4_matrix* w, const float* bias_d,
+                                 void* y_d, int y_type, void* stream);
+
+/* The first half of a gated feed-forward block in one kernel: h = act(x w_gate^T) * (x w_up^T), m x n,
+ * rounded once.  gate_d and up_d (both or neither) receive the two products, rounded to the same type,
+ * for the backward pass. */
+int int4_linear_fp4_gated_launch_async(const int4_linear_fp4_matrix* x, const int4_linear_fp4_matrix* w_gate,
+                                       const int4_linear_fp4_matrix* w_up, int activation, void* h_d, void* gate_d, void* up_d,
+                                       int h_type, void* stream);
+
+/* Backward passes, bf16 gradients, with respect to the values the operands stand for.  dx_d (m x k) and
+ * the weight gradients (n x k) may be left out with NULL, not all of them.  The workspace is 256-byte
+ * aligned device memory of at least int4_linear_fp4_grad_workspace_bytes(...) bytes, free again when the
+ * work on the stream is done; calls that can run at the same time need one each.
+ *   linear  dx = dy w            dw = dy^T x                     (dy: m x n)
+ *   gated   dg = dh up act'(gate), du = dh act(gate), rounded to bf16;
+ *           dx = dg w_gate + du w_up     dw_gate = dg^T x     dw_up = du^T x
+ * gate_d and up_d are what the forward pass kept. */
+long long int4_linear_fp4_grad_workspace_bytes(int m, int n, int k, int gated, int want_dx, int want_dw);
+int int4_linear_fp4_grad_async(const void* dy_d, const int4_linear_fp4_matrix* x, const int4_linear_fp4_matrix* w,
+                               void* dx_d, void* dw_d, void* workspace_d, long long workspace_bytes, void* stream);
+int int4_linear_fp4_gated_grad_async(const void* dh_d, const void* gate_d, const void* up_d, const int4_linear_fp4_matrix* x,
+                                     const int4_linear_fp4_matrix* w_gate, const int4_linear_fp4_matrix* w_up, int activation,
+                                     void* dx_d, void* dw_gate_d, void* dw_up_d, void* workspace_d, long long workspace_bytes,
+                                     void* stream);
+
 /* Status of the most recent call on the current device; also polls the word
  * the kernels raise when a bounded wait expires (and clears it). */
 int int4_linear_last_status(void);

@@ -34,5 +34,14 @@ from .linear import (  # noqa: F401
     PATH_LEGACY,
     PATH_SKINNY,
 )
+from .fp4 import (  # noqa: F401
+    Fp4Matrix,
+    quantize_fp4,
+    dequantize_fp4,
+    linear_fp4,
+    gated_linear_fp4,
+    linear_fp4_backward,
+    gated_linear_fp4_backward,
+)
 
 __version__ = "0.1.0"

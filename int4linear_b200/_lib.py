@@ -29,6 +29,14 @@ SYMBOLS = {
     "int4_linear_unpack_i32": (_I, [_VP, _VP, _I, _I, _VP]),
     "int4_linear_probe_stream_read": (_I, [_VP, ctypes.c_ulonglong, _VP, _VP]),
     "int4_linear_selftest_timeout": (_I, [_I]),
+    "int4_linear_fp4_scale_bytes": (_LL, [_I, _I, _I]),
+    "int4_linear_fp4_quantize_async": (_I, [_VP, _I, _LL, _VP, _VP]),
+    "int4_linear_fp4_dequantize_async": (_I, [_VP, _VP, _I, _VP]),
+    "int4_linear_fp4_launch_async": (_I, [_VP, _VP, _VP, _VP, _I, _VP]),
+    "int4_linear_fp4_gated_launch_async": (_I, [_VP, _VP, _VP, _I, _VP, _VP, _VP, _I, _VP]),
+    "int4_linear_fp4_grad_workspace_bytes": (_LL, [_I, _I, _I, _I, _I, _I]),
+    "int4_linear_fp4_grad_async": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _LL, _VP]),
+    "int4_linear_fp4_gated_grad_async": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _I, _VP, _VP, _VP, _VP, _LL, _VP]),
     "int4_linear_last_status": (_I, []),
     "int4_linear_status_string": (ctypes.c_char_p, [_I]),
     "int4_linear_set_path": (_I, [_I]),

@@ -8,6 +8,7 @@
 #include <mutex>
 
 #include "common.h"
+#include "fp4.cuh"
 #include "ptx.cuh"
 
 namespace i4l {
@@ -69,6 +70,12 @@ void report(int status, const char* what)
 }
 
 }  // namespace
+
+int record_status(int status)
+{
+    t_last_status = status;
+    return status;
+}
 
 void count_launch(int n) { g_launches.fetch_add(n); }
 
@@ -196,11 +203,29 @@ DeviceCtx* current_ctx(int* status)
     if (rc == INT4L_OK) rc = setup_tcgen05_s8(c);
     if (rc == INT4L_OK) rc = setup_skinny(c);
     if (rc == INT4L_OK) rc = setup_fewrows(c);
+    if (rc == INT4L_OK) rc = setup_fp4_gemm(c);
+    if (rc == INT4L_OK) rc = setup_grad(c);
     if (rc != INT4L_OK) { *status = rc; return nullptr; }
     c->attrs_set = true;
     g_ctx_ready[dev] = true;
     *status = INT4L_OK;
     return c;
+}
+
+int encode_tensor_map_2d(DeviceCtx* ctx, CUtensorMap* out, const void* base, int elem_bytes,
+                         uint64_t inner_elems, uint64_t rows, uint64_t row_pitch_bytes,
+                         uint32_t box_inner, uint32_t box_rows, bool swizzle128, bool swizzle64)
+{
+    const cuuint64_t dims[2] = {inner_elems, rows};
+    const cuuint64_t strides[1] = {row_pitch_bytes};
+    const cuuint32_t box[2] = {box_inner, box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    CUresult r = reinterpret_cast<EncodeTiledFn>(ctx->encode_tiled)(
+        out, elem_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_INT32 : (elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8), 2,
+        const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+        swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : (swizzle64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE),
+        CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? INT4L_OK : INT4L_ERR_CUDA;
 }
 
 int make_tensor_map_2d(DeviceCtx* ctx, CUtensorMap* out, const void* base, int elem_bytes,
@@ -218,16 +243,9 @@ int make_tensor_map_2d(DeviceCtx* ctx, CUtensorMap* out, const void* base, int e
             }
         }
     }
-    const cuuint64_t dims[2] = {inner_elems, rows};
-    const cuuint64_t strides[1] = {row_pitch_bytes};
-    const cuuint32_t box[2] = {box_inner, box_rows};
-    const cuuint32_t estr[2] = {1, 1};
-    CUresult r = reinterpret_cast<EncodeTiledFn>(ctx->encode_tiled)(
-        out, elem_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_INT32 : (elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8), 2,
-        const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-        swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : (swizzle64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE),
-        CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return INT4L_ERR_CUDA;
+    const int rc = encode_tensor_map_2d(ctx, out, base, elem_bytes, inner_elems, rows, row_pitch_bytes, box_inner, box_rows,
+                                        swizzle128, swizzle64);
+    if (rc != INT4L_OK) return rc;
     // A tensor map describes addresses and shapes only, never contents, so a remembered one stays
     // valid for as long as the same pointer denotes an allocation of at least that extent.
     std::lock_guard<std::mutex> lock(g_tm_mutex);

@@ -1,0 +1,232 @@
+// C-ABI layer of the microscaled 4-bit floating-point operators (include/int4linear_b200.h): argument checks,
+// workspace layout of the backward passes, and the order of their launches.
+#include "fp4.cuh"
+
+using namespace i4l;
+
+namespace {
+
+bool misaligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }
+
+int take_matrix(const int4_linear_fp4_matrix* q, Fp4* out)
+{
+    if (!q || !q->codes || !q->scales || q->rows <= 0 || q->k <= 0) return INT4L_ERR_INVALID_ARG;
+    if (q->format != INT4L_FP4_MX && q->format != INT4L_FP4_NV) return INT4L_ERR_INVALID_ARG;
+    if (q->format == INT4L_FP4_MX && q->tensor_scale) return INT4L_ERR_INVALID_ARG;
+    if (q->k % 32 != 0) return INT4L_ERR_UNSUPPORTED;
+    if (misaligned(q->codes, 16) || misaligned(q->scales, 16) || misaligned(q->tensor_scale, 4)) return INT4L_ERR_MISALIGNED;
+    out->codes = static_cast<const uint8_t*>(q->codes);
+    out->scales = static_cast<const uint8_t*>(q->scales);
+    out->tensor_scale = q->tensor_scale;
+    out->rows = q->rows;
+    out->k = q->k;
+    out->block16 = q->format == INT4L_FP4_NV;
+    return INT4L_OK;
+}
+
+int element_bytes(int type) { return type == INT4L_TYPE_F32 ? 4 : 2; }
+
+// x[m x k] and one or two w[n x k] of one format.
+int take_operands(const int4_linear_fp4_matrix* x, const int4_linear_fp4_matrix* w, const int4_linear_fp4_matrix* w_up, bool gated, Fp4Problem* p)
+{
+    int rc = take_matrix(x, &p->x);
+    if (rc == INT4L_OK) rc = take_matrix(w, &p->w);
+    if (rc == INT4L_OK && gated) rc = take_matrix(w_up, &p->w_up);
+    if (rc != INT4L_OK) return rc;
+    if (p->x.k != p->w.k || p->x.block16 != p->w.block16) return INT4L_ERR_INVALID_ARG;
+    if (gated && (p->w_up.k != p->x.k || p->w_up.rows != p->w.rows || p->w_up.block16 != p->x.block16)) return INT4L_ERR_INVALID_ARG;
+    p->gated = gated;
+    p->m = p->x.rows;
+    p->n = p->w.rows;
+    p->k = p->x.k;
+    return INT4L_OK;
+}
+
+bool bad_act(int act) { return act != INT4L_ACT_SILU && act != INT4L_ACT_GELU && act != INT4L_ACT_GELU_TANH; }
+
+// Pieces of a backward pass's workspace, in order, each on a 256-byte boundary.
+struct GradLayout {
+    long long d0 = 0, d1 = 0, w0 = 0, w1 = 0, x = 0, bytes = 0, ld = 0;
+};
+GradLayout grad_layout(long long m, long long n, long long k, bool gated, bool want_dx, bool want_dw)
+{
+    GradLayout l;
+    l.ld = (n + 7) / 8 * 8;
+    auto piece = [&](long long bytes) { const long long at = l.bytes; l.bytes += (bytes + 255) / 256 * 256; return at; };
+    if (gated) { l.d0 = piece(m * l.ld * 2); l.d1 = piece(m * l.ld * 2); }
+    else if (n % 8 != 0) l.d0 = piece(m * l.ld * 2);
+    if (want_dx) { l.w0 = piece(n * k * 2); if (gated) l.w1 = piece(n * k * 2); }
+    if (want_dw) l.x = piece(m * k * 2);
+    return l;
+}
+
+}  // namespace
+
+extern "C" {
+
+long long int4_linear_fp4_scale_bytes(int rows, int k, int format)
+{
+    if (rows <= 0 || k <= 0 || k % 32 != 0 || (format != INT4L_FP4_MX && format != INT4L_FP4_NV)) return -INT4L_ERR_INVALID_ARG;
+    return (rows + 127ll) / 128 * fp4_ktiles(k, format == INT4L_FP4_NV) * kScaleTileBytes;
+}
+
+int int4_linear_fp4_quantize_async(const void* src_d, int src_type, long long src_pitch, const int4_linear_fp4_matrix* dst, void* stream)
+{
+    Fp4 d;
+    int rc = take_matrix(dst, &d);
+    if (rc == INT4L_OK && (!src_d || src_type < INT4L_TYPE_BF16 || src_type > INT4L_TYPE_F32 || src_pitch < d.k)) rc = INT4L_ERR_INVALID_ARG;
+    if (rc == INT4L_OK && misaligned(src_d, element_bytes(src_type))) rc = INT4L_ERR_MISALIGNED;
+    if (rc != INT4L_OK) return record_status(rc);
+    DeviceCtx* ctx = current_ctx(&rc);
+    if (ctx) rc = launch_fp4_quantize(ctx, src_d, src_type, src_pitch, d, static_cast<cudaStream_t>(stream));
+    return record_status(rc);
+}
+
+int int4_linear_fp4_dequantize_async(const int4_linear_fp4_matrix* src, void* dst_d, int dst_type, void* stream)
+{
+    Fp4 s;
+    int rc = take_matrix(src, &s);
+    if (rc == INT4L_OK && (!dst_d || dst_type < INT4L_TYPE_BF16 || dst_type > INT4L_TYPE_F32)) rc = INT4L_ERR_INVALID_ARG;
+    if (rc == INT4L_OK && misaligned(dst_d, 16)) rc = INT4L_ERR_MISALIGNED;
+    if (rc != INT4L_OK) return record_status(rc);
+    DeviceCtx* ctx = current_ctx(&rc);
+    if (ctx) rc = launch_fp4_dequantize(ctx, s, dst_d, dst_type, true, static_cast<cudaStream_t>(stream));
+    return record_status(rc);
+}
+
+int int4_linear_fp4_launch_async(const int4_linear_fp4_matrix* x, const int4_linear_fp4_matrix* w, const float* bias_d,
+                                 void* y_d, int y_type, void* stream)
+{
+    Fp4Problem p;
+    int rc = take_operands(x, w, nullptr, false, &p);
+    if (rc == INT4L_OK && (!y_d || (y_type != INT4L_TYPE_BF16 && y_type != INT4L_TYPE_F16))) rc = INT4L_ERR_INVALID_ARG;
+    if (rc == INT4L_OK && (misaligned(y_d, 16) || misaligned(bias_d, 4))) rc = INT4L_ERR_MISALIGNED;
+    if (rc != INT4L_OK) return record_status(rc);
+    DeviceCtx* ctx = current_ctx(&rc);
+    if (!ctx) return record_status(rc);
+    p.bias = bias_d;
+    p.y = y_d;
+    p.fp16 = y_type == INT4L_TYPE_F16;
+    return record_status(launch_fp4_gemm(ctx, p, static_cast<cudaStream_t>(stream)));
+}
+
+int int4_linear_fp4_gated_launch_async(const int4_linear_fp4_matrix* x, const int4_linear_fp4_matrix* w_gate,
+                                       const int4_linear_fp4_matrix* w_up, int activation, void* h_d, void* gate_d, void* up_d,
+                                       int h_type, void* stream)
+{
+    Fp4Problem p;
+    int rc = take_operands(x, w_gate, w_up, true, &p);
+    if (rc == INT4L_OK && (!h_d || !gate_d != !up_d || bad_act(activation) || (h_type != INT4L_TYPE_BF16 && h_type != INT4L_TYPE_F16)))
+        rc = INT4L_ERR_INVALID_ARG;
+    if (rc == INT4L_OK && (misaligned(h_d, 16) || misaligned(gate_d, 16) || misaligned(up_d, 16))) rc = INT4L_ERR_MISALIGNED;
+    if (rc != INT4L_OK) return record_status(rc);
+    DeviceCtx* ctx = current_ctx(&rc);
+    if (!ctx) return record_status(rc);
+    p.act = activation;
+    p.y = h_d;
+    p.keep_gate = gate_d;
+    p.keep_up = up_d;
+    p.fp16 = h_type == INT4L_TYPE_F16;
+    return record_status(launch_fp4_gemm(ctx, p, static_cast<cudaStream_t>(stream)));
+}
+
+long long int4_linear_fp4_grad_workspace_bytes(int m, int n, int k, int gated, int want_dx, int want_dw)
+{
+    if (m <= 0 || n <= 0 || k <= 0) return -INT4L_ERR_INVALID_ARG;
+    return grad_layout(m, n, k, gated != 0, want_dx != 0, want_dw != 0).bytes;
+}
+
+int int4_linear_fp4_grad_async(const void* dy_d, const int4_linear_fp4_matrix* x, const int4_linear_fp4_matrix* w,
+                               void* dx_d, void* dw_d, void* workspace_d, long long workspace_bytes, void* stream)
+{
+    Fp4Problem p;
+    int rc = take_operands(x, w, nullptr, false, &p);
+    if (rc == INT4L_OK && (!dy_d || (!dx_d && !dw_d))) rc = INT4L_ERR_INVALID_ARG;
+    if (rc == INT4L_OK && (misaligned(dy_d, 16) || misaligned(dx_d, 16) || misaligned(dw_d, 16) || misaligned(workspace_d, 256))) rc = INT4L_ERR_MISALIGNED;
+    if (rc != INT4L_OK) return record_status(rc);
+    const GradLayout l = grad_layout(p.m, p.n, p.k, false, dx_d != nullptr, dw_d != nullptr);
+    if (!workspace_d || workspace_bytes < l.bytes) return record_status(INT4L_ERR_INVALID_ARG);
+    DeviceCtx* ctx = current_ctx(&rc);
+    if (!ctx) return record_status(rc);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    uint8_t* ws = static_cast<uint8_t*>(workspace_d);
+    GradProduct g;
+    g.m = p.m; g.n = p.n; g.k = p.k; g.ld = l.ld;
+    g.d0 = dy_d;
+    if (p.n % 8 != 0) {  // TMA needs a 16-byte row pitch
+        if (cudaMemcpy2DAsync(ws + l.d0, l.ld * 2, dy_d, p.n * 2ull, p.n * 2ull, p.m, cudaMemcpyDeviceToDevice, s) != cudaSuccess) {
+            cudaGetLastError();
+            return record_status(INT4L_ERR_CUDA);
+        }
+        g.d0 = ws + l.d0;
+    }
+    if (rc == INT4L_OK && dx_d) {
+        rc = launch_fp4_dequantize(ctx, p.w, ws + l.w0, INT4L_TYPE_BF16, false, s);
+        GradProduct d = g;
+        d.b0 = ws + l.w0;
+        d.out = dx_d;
+        d.num = p.w.tensor_scale;
+        if (rc == INT4L_OK) rc = launch_grad_product(ctx, d, s);
+    }
+    if (rc == INT4L_OK && dw_d) {
+        rc = launch_fp4_dequantize(ctx, p.x, ws + l.x, INT4L_TYPE_BF16, false, s);
+        GradProduct d = g;
+        d.weight = true;
+        d.b0 = ws + l.x;
+        d.out = dw_d;
+        d.num = p.x.tensor_scale;
+        if (rc == INT4L_OK) rc = launch_grad_product(ctx, d, s);
+    }
+    return record_status(rc);
+}
+
+int int4_linear_fp4_gated_grad_async(const void* dh_d, const void* gate_d, const void* up_d, const int4_linear_fp4_matrix* x,
+                                     const int4_linear_fp4_matrix* w_gate, const int4_linear_fp4_matrix* w_up, int activation,
+                                     void* dx_d, void* dw_gate_d, void* dw_up_d, void* workspace_d, long long workspace_bytes,
+                                     void* stream)
+{
+    Fp4Problem p;
+    int rc = take_operands(x, w_gate, w_up, true, &p);
+    if (rc == INT4L_OK && (!dh_d || !gate_d || !up_d || (!dx_d && !dw_gate_d) || !dw_gate_d != !dw_up_d || bad_act(activation))) rc = INT4L_ERR_INVALID_ARG;
+    if (rc == INT4L_OK && (misaligned(dh_d, 2) || misaligned(gate_d, 2) || misaligned(up_d, 2) || misaligned(dx_d, 16) ||
+                           misaligned(dw_gate_d, 16) || misaligned(dw_up_d, 16) || misaligned(workspace_d, 256)))
+        rc = INT4L_ERR_MISALIGNED;
+    if (rc != INT4L_OK) return record_status(rc);
+    const GradLayout l = grad_layout(p.m, p.n, p.k, true, dx_d != nullptr, dw_gate_d != nullptr);
+    if (!workspace_d || workspace_bytes < l.bytes) return record_status(INT4L_ERR_INVALID_ARG);
+    DeviceCtx* ctx = current_ctx(&rc);
+    if (!ctx) return record_status(rc);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    uint8_t* ws = static_cast<uint8_t*>(workspace_d);
+    // dg and du carry their weight's tensor scale, so that dx is one contraction over both; the weight
+    // gradients take it out again.
+    rc = launch_gate_backward(ctx, dh_d, gate_d, up_d, ws + l.d0, ws + l.d1, activation, p.w.tensor_scale, p.w_up.tensor_scale,
+                              p.m, p.n, l.ld, s);
+    GradProduct g;
+    g.m = p.m; g.n = p.n; g.k = p.k; g.ld = l.ld;
+    if (rc == INT4L_OK && dx_d) {
+        rc = launch_fp4_dequantize(ctx, p.w, ws + l.w0, INT4L_TYPE_BF16, false, s);
+        if (rc == INT4L_OK) rc = launch_fp4_dequantize(ctx, p.w_up, ws + l.w1, INT4L_TYPE_BF16, false, s);
+        GradProduct d = g;
+        d.d0 = ws + l.d0; d.d1 = ws + l.d1;
+        d.b0 = ws + l.w0; d.b1 = ws + l.w1;
+        d.out = dx_d;
+        if (rc == INT4L_OK) rc = launch_grad_product(ctx, d, s);
+    }
+    if (rc == INT4L_OK && dw_gate_d) {
+        rc = launch_fp4_dequantize(ctx, p.x, ws + l.x, INT4L_TYPE_BF16, false, s);
+        for (int i = 0; i < 2 && rc == INT4L_OK; ++i) {
+            GradProduct d = g;
+            d.weight = true;
+            d.d0 = ws + (i ? l.d1 : l.d0);
+            d.b0 = ws + l.x;
+            d.out = i ? dw_up_d : dw_gate_d;
+            d.num = p.x.tensor_scale;
+            d.den = i ? p.w_up.tensor_scale : p.w.tensor_scale;
+            rc = launch_grad_product(ctx, d, s);
+        }
+    }
+    return record_status(rc);
+}
+
+}  // extern "C"

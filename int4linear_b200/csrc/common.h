@@ -94,6 +94,9 @@ struct DeviceCtx {
     bool attrs_set = false;
 };
 
+// Records a call's status for int4_linear_last_status() and returns it.
+int record_status(int status);
+
 // Returns the context of the current device (nullptr + status on failure).
 DeviceCtx* current_ctx(int* status);
 
@@ -104,6 +107,11 @@ DeviceCtx* current_ctx(int* status);
 int make_tensor_map_2d(DeviceCtx* ctx, CUtensorMap* out, const void* base, int elem_bytes,
                        uint64_t inner_elems, uint64_t rows, uint64_t row_pitch_bytes,
                        uint32_t box_inner, uint32_t box_rows, bool swizzle128, bool swizzle64 = false);
+
+// The same without looking for, or keeping, an earlier encoding.
+int encode_tensor_map_2d(DeviceCtx* ctx, CUtensorMap* out, const void* base, int elem_bytes,
+                         uint64_t inner_elems, uint64_t rows, uint64_t row_pitch_bytes,
+                         uint32_t box_inner, uint32_t box_rows, bool swizzle128, bool swizzle64 = false);
 
 // Destinations of the gathering GEMM: the full-width Y (m x n_total int32) of every rank.
 struct GatherDst {

@@ -274,4 +274,59 @@ __device__ __forceinline__ void drain_accumulator_scaled_tma(uint32_t t_addr, in
     }
 }
 
+// Two floats -> two 16-bit floats (round to nearest even), the first in the low half.
+__device__ __forceinline__ uint32_t pack16(float a, float b, int fp16)
+{
+    if (fp16) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// One warp writes 32 rows x 64 columns of 16-bit values (two per register, lane = row): through its staging
+// tile (128-byte swizzle) and one TMA store, which clips the tails; or, where the row pitch forbids that
+// (n % 8 != 0), from the staging tile row by row, 32 neighbouring values per store instruction.
+__device__ __forceinline__ void store_block(const uint32_t (&h)[32], uint32_t stg, const CUtensorMap* map, unsigned short* out,
+                                            int row0, int col0, int m, int n, int tma_store, int lane)
+{
+    if (row0 >= m || col0 >= n) return;
+    if (lane == 0) tma_store_wait_read<0>();
+    __syncwarp();
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+        sts128(stg + lane * 128 + ((q ^ (lane & 7)) << 4), make_uint4(h[4 * q], h[4 * q + 1], h[4 * q + 2], h[4 * q + 3]));
+    if (tma_store) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+            tma_store_2d(map, stg, col0, row0);
+            tma_store_commit();
+        }
+    } else {
+        __syncwarp();
+        const int rows = min(32, m - row0);
+#pragma unroll 1
+        for (int r = 0; r < rows; ++r) {
+            unsigned short* dst = out + static_cast<size_t>(row0 + r) * n + col0;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int c = lane + 32 * e;
+                uint16_t v;
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(stg + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2));
+                if (col0 + c < n) dst[c] = v;
+            }
+        }
+        __syncwarp();
+    }
+}
+
+// 64 consecutive accumulator columns of this thread's lane (asynchronous until tmem_ld_wait()).
+__device__ __forceinline__ void load64(uint32_t taddr, uint32_t (&v)[64])
+{
+    tmem_ld_32x32(taddr, *reinterpret_cast<uint32_t (*)[32]>(v));
+    tmem_ld_32x32(taddr + 32, *reinterpret_cast<uint32_t (*)[32]>(v + 32));
+}
+
 }  // namespace i4l

@@ -1,0 +1,46 @@
+// Activations of the gated feed-forward block and their derivatives, in fp32.
+//     silu       g s(g)                 s the logistic function
+//     gelu       g P(g)                 P the normal distribution function
+//     gelu_tanh  g s(2 z), z = sqrt(2/pi) (g + 0.044715 g^3)   ( = g (1 + tanh z) / 2 )
+// Each is written so that nothing cancels for large negative g, where act(g) goes to 0.
+#pragma once
+
+#include "fp4.cuh"
+
+namespace i4l {
+
+constexpr float kGeluC = 0.7978845608028654f;  // sqrt(2 / pi)
+constexpr float kGeluA = 0.044715f;
+
+__device__ __forceinline__ float logistic(float v) { return 1.0f / (1.0f + __expf(-v)); }
+__device__ __forceinline__ float normal_cdf(float v) { return 0.5f * erfcf(-0.7071067811865476f * v); }
+
+template <int kAct>
+__device__ __forceinline__ float gate_act(float g)
+{
+    if constexpr (kAct == kActSilu) return g * logistic(g);
+    else if constexpr (kAct == kActGelu) return g * normal_cdf(g);
+    else return g * logistic(2.0f * kGeluC * (g + kGeluA * g * g * g));
+}
+
+// act(g) and act'(g).
+template <int kAct>
+__device__ __forceinline__ void gate_act_slope(float g, float& act, float& slope)
+{
+    if constexpr (kAct == kActSilu) {
+        const float s = logistic(g);
+        act = g * s;
+        slope = s * (1.0f + g * logistic(-g));
+    } else if constexpr (kAct == kActGelu) {
+        const float p = normal_cdf(g);
+        act = g * p;
+        slope = p + g * 0.3989422804014327f * __expf(-0.5f * g * g);
+    } else {
+        const float z2 = 2.0f * kGeluC * (g + kGeluA * g * g * g);
+        const float s = logistic(z2);
+        act = g * s;
+        slope = s * (1.0f + g * logistic(-z2) * 2.0f * kGeluC * (1.0f + 3.0f * kGeluA * g * g));
+    }
+}
+
+}  // namespace i4l

@@ -208,6 +208,14 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* m, 
         : "memory");
 }
 
+// Untiled bulk load global -> this CTA's shared memory: both addresses 16-byte aligned, bytes a multiple of 16.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
+        : "memory");
+}
+
 // 2-D tiled store shared -> global (bulk-group completion).  Elements of the
 // box that fall outside the tensor are not written.
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* m, uint32_t src, int c0, int c1) {
@@ -322,6 +330,98 @@ __device__ __forceinline__ void umma_i8_a_tmem(uint32_t d_tmem, uint32_t a_tmem,
         "tcgen05.mma.cta_group::1.kind::i8 [%0], [%1], %2, %3, p;\n\t"
         "}\n" ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
+}
+
+// Instruction descriptor for the block-scaled 4-bit kinds: A and B e2m1 (format 1), both K-major, fp32
+// accumulator, dense, K = 64 per instruction.
+//   bits 4-5 / 29-30 scale-factor id of B / A; 7-9, 10-12 operand formats (1 = e2m1);
+//   17-22 N>>3; 23 scale type (0 = ue4m3, 1 = ue8m0); 24-28 M>>4.
+// A scale-factor id names the first byte an instruction uses of each 32-bit scale word (0 or 2 when a
+// word serves two instructions: mxfp4; 0 when it serves one: nvfp4).
+__host__ __device__ constexpr uint32_t umma_idesc_fp4(int m, int n, bool ue8m0, uint32_t sf_id) {
+    return (sf_id << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
+           (ue8m0 ? 1u << 23 : 0u) | (static_cast<uint32_t>(m >> 4) << 24) | (sf_id << 29);
+}
+
+// D[tmem] (+)= (A[smem] scaled) * (B[smem] scaled)^T, K = 64, scales in tensor memory (a row's scale word in
+// lane row % 32, column row / 32, the 32 lanes repeated in all four quarters).  Issued by ONE thread.
+// kBlock16: nvfp4 (a ue4m3 scale per 16 elements), else mxfp4 (a ue8m0 scale per 32).
+template <int kCtaGroup, bool kBlock16>
+__device__ __forceinline__ void umma_fp4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                         uint32_t sfa_tmem, uint32_t sfb_tmem, uint32_t accumulate) {
+#define I4L_UMMA_FP4(GROUP, KIND)                                                                        \
+    asm volatile(                                                                                        \
+        "{\n\t"                                                                                          \
+        ".reg .pred p;\n\t"                                                                              \
+        "setp.ne.b32 p, %6, 0;\n\t"                                                                      \
+        "tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, [%4], [%5], p;\n\t"           \
+        "}\n" ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem),         \
+        "r"(accumulate) : "memory")
+    if constexpr (kCtaGroup == 1) {
+        if constexpr (kBlock16) I4L_UMMA_FP4("1", "mxf4nvf4.block_scale.scale_vec::4X");
+        else I4L_UMMA_FP4("1", "mxf4.block_scale.scale_vec::2X");
+    } else {
+        if constexpr (kBlock16) I4L_UMMA_FP4("2", "mxf4nvf4.block_scale.scale_vec::4X");
+        else I4L_UMMA_FP4("2", "mxf4.block_scale.scale_vec::2X");
+    }
+#undef I4L_UMMA_FP4
+}
+
+// Shared-memory descriptor of one 512-byte scale tile (32 rows of 16 bytes, no swizzle: 8-row groups of
+// 128 bytes that follow one another) for tcgen05.cp 32x128b.
+__device__ __forceinline__ uint64_t scale_tile_desc(uint32_t smem_addr) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+    d |= static_cast<uint64_t>(128 >> 4) << 32;
+    d |= static_cast<uint64_t>(1) << 46;
+    return d;
+}
+// Copies one scale tile into 4 columns of tensor memory (repeated in the four lane quarters).  Issued by the
+// thread that issues the UMMAs reading it: copies and UMMAs of one thread are executed in order.
+template <int kCtaGroup>
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
+    if constexpr (kCtaGroup == 1)
+        asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    else
+        asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+// Instruction descriptor for kind::f16 with bfloat16 operands and an fp32 accumulator.
+//   bits 4-5 D format (1 = f32); 7-9, 10-12 operand formats (1 = bf16); 15/16 A/B major (0 = K, 1 = MN);
+//   17-22 N>>3; 24-28 M>>4.
+__host__ __device__ constexpr uint32_t umma_idesc_bf16(int m, int n, bool a_mn_major, bool b_mn_major) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (a_mn_major ? 1u << 15 : 0u) | (b_mn_major ? 1u << 16 : 0u) |
+           (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+template <int kCtaGroup>
+__device__ __forceinline__ void umma_bf16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (kCtaGroup == 1)
+        asm volatile(
+            "{\n\t"
+            ".reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+            "}\n" ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t"
+            ".reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t"
+            "}\n" ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+            : "memory");
+}
+// Descriptor of an MN-major 16-bit operand with the 128-byte swizzle: atoms of 64 (MN) x 8 (K) elements,
+// 1024 bytes; atoms follow one another along K, `chunk_bytes` apart along MN.
+__device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t smem_addr, uint32_t chunk_bytes) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+    d |= static_cast<uint64_t>(chunk_bytes >> 4) << 16;
+    d |= static_cast<uint64_t>(1024 >> 4) << 32;
+    d |= static_cast<uint64_t>(1) << 46;
+    d |= static_cast<uint64_t>(2) << 61;
+    return d;
 }
 
 // Arrive once on `bar` when every UMMA this thread issued so far has finished
