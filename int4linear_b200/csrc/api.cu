@@ -220,8 +220,11 @@ int encode_tensor_map_2d(DeviceCtx* ctx, CUtensorMap* out, const void* base, int
     const cuuint64_t strides[1] = {row_pitch_bytes};
     const cuuint32_t box[2] = {box_inner, box_rows};
     const cuuint32_t estr[2] = {1, 1};
+    const CUtensorMapDataType type = elem_bytes == 8 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT64
+                                   : elem_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_INT32
+                                   : elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
     CUresult r = reinterpret_cast<EncodeTiledFn>(ctx->encode_tiled)(
-        out, elem_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_INT32 : (elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8), 2,
+        out, type, 2,
         const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
         swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : (swizzle64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE),
         CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);

@@ -101,7 +101,7 @@ int record_status(int status);
 DeviceCtx* current_ctx(int* status);
 
 // Builds a 2-D tiled tensor map over a row-major byte/word matrix.
-//   elem_bytes 1 -> UINT8 elements, 4 -> INT32 elements.
+//   elem_bytes 1 -> UINT8 elements, 2 -> UINT16, 4 -> INT32, 8 -> 64-bit.
 //   swizzle128 selects CU_TENSOR_MAP_SWIZZLE_128B (inner box must be 128 B),
 //   swizzle64 CU_TENSOR_MAP_SWIZZLE_64B (inner box 64 B).
 int make_tensor_map_2d(DeviceCtx* ctx, CUtensorMap* out, const void* base, int elem_bytes,

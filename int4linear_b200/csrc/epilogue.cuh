@@ -275,9 +275,10 @@ __device__ __forceinline__ void drain_accumulator_scaled_tma(uint32_t t_addr, in
 }
 
 // Two floats -> two 16-bit floats (round to nearest even), the first in the low half.
-__device__ __forceinline__ uint32_t pack16(float a, float b, int fp16)
+template <bool kHalf>
+__device__ __forceinline__ uint32_t pack16(float a, float b)
 {
-    if (fp16) {
+    if constexpr (kHalf) {
         const __half2 h = __floats2half2_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&h);
     }

@@ -12,7 +12,9 @@ namespace i4l {
 constexpr float kGeluC = 0.7978845608028654f;  // sqrt(2 / pi)
 constexpr float kGeluA = 0.044715f;
 
-__device__ __forceinline__ float logistic(float v) { return 1.0f / (1.0f + __expf(-v)); }
+// Two ulp of exp and of the reciprocal: the result is rounded to 16 bits.  (exp overflows to infinity for
+// v < -88, whose reciprocal is the 0 that is wanted.)
+__device__ __forceinline__ float logistic(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
 __device__ __forceinline__ float normal_cdf(float v) { return 0.5f * erfcf(-0.7071067811865476f * v); }
 
 template <int kAct>

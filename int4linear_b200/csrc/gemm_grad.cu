@@ -199,7 +199,7 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
                 load64(t_addr + c, v);
                 tmem_ld_wait();
 #pragma unroll
-                for (int j = 0; j < 32; ++j) h[j] = pack16(__uint_as_float(v[2 * j]) * alpha, __uint_as_float(v[2 * j + 1]) * alpha, 0);
+                for (int j = 0; j < 32; ++j) h[j] = pack16<false>(__uint_as_float(v[2 * j]) * alpha, __uint_as_float(v[2 * j + 1]) * alpha);
                 const uint32_t stg = stage0 + (chunk_no & 1u) * kStoreStage;
                 if (lane == 0) tma_store_wait_read<1>();
                 __syncwarp();
