@@ -168,18 +168,18 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
 
     if (warp == 0) {
         // ------------------------------------------------------ TMA producer
-        if (lane == 0) {
-            uint32_t it = 0;
-            bool alive = true;
-            for (int tile = worker; alive && tile < num_tiles; tile += workers) {
-                int tm, tn;
-                tile_coord(tile, tm, tn);
-                const int group_x = tm * 2 + static_cast<int>(cta_rank);
-                const CUtensorMap* map_w = (kGated && cta_rank) ? &tm_w_up : &tm_w;
-                const int group_w = kGated ? tn : tn * 2 + static_cast<int>(cta_rank);
-                for (int kb = 0; kb < steps; ++kb, ++it) {
-                    const uint32_t s = it % S, r = it / S;
-                    if (!mbar_wait(empty(s), (r & 1u) ^ 1u, abort_flag)) { alive = false; break; }
+        uint32_t it = 0;
+        bool alive = true;
+        for (int tile = worker; alive && tile < num_tiles; tile += workers) {
+            int tm, tn;
+            tile_coord(tile, tm, tn);
+            const int group_x = tm * 2 + static_cast<int>(cta_rank);
+            const CUtensorMap* map_w = (kGated && cta_rank) ? &tm_w_up : &tm_w;
+            const int group_w = kGated ? tn : tn * 2 + static_cast<int>(cta_rank);
+            for (int kb = 0; kb < steps; ++kb, ++it) {
+                const uint32_t s = it % S, r = it / S;
+                if (!mbar_wait_warp(empty(s), (r & 1u) ^ 1u, abort_flag)) { alive = false; break; }
+                if (elect_one()) {
                     // CTA 1's bytes may be counted before CTA 0 announces them: the phase cannot end before the
                     // announcement, which is its one arrival.  What lies outside a matrix is read as 0 and counted.
                     if (cta_rank == 0) mbar_expect_tx(full(s), 2 * G::kStage);
@@ -196,9 +196,9 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
                         tma_load_2d_pair(dst + G::kCodeBytes + G::kScaleBytesA, &tm_sw, bar, sc, tn * 2);  // two groups
                     }
                 }
+                __syncwarp();
             }
         }
-        __syncwarp();
     } else if (warp == 1) {
         if (cta_rank == 0) {
             // ----------------------------------------------------- UMMA issuer

@@ -12,7 +12,7 @@
 // The products are one persistent kernel, a CTA pair per 256 x 256 tile (tcgen05.mma kind::f16, cta_group::2),
 // two accumulators in tensor memory so that the epilogue overlaps the next tile:
 //     warp 0      TMA, steps of 64 along the contraction, into 128-byte-swizzled slots
-//     warp 1      UMMA issue (CTA 0 for both); in CTA 1 "my tiles have landed"
+//     warp 1      UMMA issue (CTA 0 for both)
 //     warps 2-5   epilogue: scale, round to bf16, staged TMA stores
 // No operand is ever transposed: where the contraction runs down the rows of a matrix (w and x always, dy for
 // dw), its tile is read as it lies and the UMMA takes it MN-major.
@@ -31,7 +31,7 @@ constexpr int kStages = 6;
 constexpr int kStage = 2 * 128 * 128;          // A and B tile of one CTA, 16 KB each
 constexpr int kChunk = kStepK * 128;           // MN-major: 64 columns x 64 rows
 constexpr int kStoreStage = 4096;              // per warp and buffer
-constexpr int kNumBarriers = 3 * kStages + 4;
+constexpr int kNumBarriers = 2 * kStages + 4;
 constexpr int kSmemBytes = 1024 + kStages * kStage + 4 * 2 * kStoreStage + kNumBarriers * 8 + 16;
 static_assert(kSmemBytes <= 232448, "shared memory budget");
 
@@ -58,11 +58,10 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
     const uint32_t ring = base;
     const uint32_t st_base = ring + S * kStage;
     const uint32_t bar_base = st_base + 4 * 2 * kStoreStage;
-    auto full      = [&](int i) { return bar_base + 8u * i; };
-    auto empty     = [&](int i) { return bar_base + 8u * (S + i); };
-    auto peer_full = [&](int i) { return bar_base + 8u * (2 * S + i); };
-    auto tm_full   = [&](int i) { return bar_base + 8u * (3 * S + i); };
-    auto tm_empty  = [&](int i) { return bar_base + 8u * (3 * S + 2 + i); };
+    auto full     = [&](int i) { return bar_base + 8u * i; };
+    auto empty    = [&](int i) { return bar_base + 8u * (S + i); };
+    auto tm_full  = [&](int i) { return bar_base + 8u * (2 * S + i); };
+    auto tm_empty  = [&](int i) { return bar_base + 8u * (2 * S + 2 + i); };
     const uint32_t misc_off = (bar_base - base) + 8u * kNumBarriers;
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gbase + misc_off);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + misc_off + 4);
@@ -73,7 +72,7 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
     const int workers = static_cast<int>(cluster_count_x());
 
     if (tid == 0) {
-        for (int i = 0; i < S; ++i) { mbar_init(full(i), 1); mbar_init(empty(i), 1); mbar_init(peer_full(i), 1); }
+        for (int i = 0; i < S; ++i) { mbar_init(full(i), 1); mbar_init(empty(i), 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(tm_full(i), 1); mbar_init(tm_empty(i), 4 * 2); }
         *abort_flag = 0;
         mbar_init_fence();
@@ -105,70 +104,66 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
 
     if (warp == 0) {
         // ------------------------------------------------------ TMA producer
-        if (lane == 0) {
-            uint32_t it = 0;
-            bool alive = true;
-            for (int tile = worker; alive && tile < num_tiles; tile += workers) {
-                int tm, tn;
-                tile_coord(tile, tm, tn);
-                const int row = (tm * 2 + static_cast<int>(cta_rank)) * kBM;
-                const int col = tn * kBN + static_cast<int>(cta_rank) * 128;
-                for (int st = 0; st < steps; ++st, ++it) {
-                    const uint32_t s = it % S, r = it / S;
-                    if (!mbar_wait(empty(s), (r & 1u) ^ 1u, abort_flag)) { alive = false; break; }
-                    mbar_expect_tx(full(s), kStage);
+        uint32_t it = 0;
+        bool alive = true;
+        for (int tile = worker; alive && tile < num_tiles; tile += workers) {
+            int tm, tn;
+            tile_coord(tile, tm, tn);
+            const int row = (tm * 2 + static_cast<int>(cta_rank)) * kBM;
+            const int col = tn * kBN + static_cast<int>(cta_rank) * 128;
+            for (int st = 0; st < steps; ++st, ++it) {
+                const uint32_t s = it % S, r = it / S;
+                if (!mbar_wait_warp(empty(s), (r & 1u) ^ 1u, abort_flag)) { alive = false; break; }
+                if (elect_one()) {
+                    // Both CTAs' loads are counted on CTA 0's barrier (which cannot complete before this announcement).
+                    if (cta_rank == 0) mbar_expect_tx(full(s), 2 * kStage);
+                    const uint32_t bar = cluster_address(full(s), 0);
                     const uint32_t dst = ring + s * kStage;
                     const bool second = st >= a.steps;
                     const int k0 = (second ? st - a.steps : st) * kStepK;
                     const CUtensorMap* ta = second ? &tm_a1 : &tm_a0;
                     const CUtensorMap* tb = second ? &tm_b1 : &tm_b0;
                     if constexpr (kWeight) {
-                        tma_load_2d(dst, ta, full(s), row, k0);
-                        tma_load_2d(dst + kChunk, ta, full(s), row + 64, k0);
+                        tma_load_2d_pair(dst, ta, bar, row, k0);
+                        tma_load_2d_pair(dst + kChunk, ta, bar, row + 64, k0);
                     } else {
-                        tma_load_2d(dst, ta, full(s), k0, row);
+                        tma_load_2d_pair(dst, ta, bar, k0, row);
                     }
-                    tma_load_2d(dst + 2 * kChunk, tb, full(s), col, k0);
-                    tma_load_2d(dst + 3 * kChunk, tb, full(s), col + 64, k0);
+                    tma_load_2d_pair(dst + 2 * kChunk, tb, bar, col, k0);
+                    tma_load_2d_pair(dst + 3 * kChunk, tb, bar, col + 64, k0);
                 }
+                __syncwarp();
             }
         }
-        __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0 && cta_rank == 0) {
+        if (cta_rank == 0) {
             // ----------------------------------------------------- UMMA issuer
+            // The warp walks the ring together and one elected thread issues.
             constexpr uint32_t idesc = umma_idesc_bf16(2 * kBM, kBN, kWeight, true);
             uint32_t it = 0, local_tile = 0;
             bool alive = true;
             for (int tile = worker; alive && tile < num_tiles; tile += workers, ++local_tile) {
                 const uint32_t buf = local_tile & 1u, br = local_tile >> 1;
-                if (!mbar_wait(tm_empty(buf), (br & 1u) ^ 1u, abort_flag)) { alive = false; break; }
+                if (!mbar_wait_warp(tm_empty(buf), (br & 1u) ^ 1u, abort_flag)) break;
                 tc_fence_after_sync();
                 const uint32_t d_tmem = tmem_base + buf * kBN;
                 for (int st = 0; st < steps; ++st, ++it) {
                     const uint32_t s = it % S, r = it / S;
-                    if (!mbar_wait(full(s), r & 1u, abort_flag) || !mbar_wait(peer_full(s), r & 1u, abort_flag)) { alive = false; break; }
+                    if (!mbar_wait_warp(full(s), r & 1u, abort_flag)) { alive = false; break; }
                     tc_fence_after_sync();
                     const uint32_t a_addr = ring + s * kStage;
                     const uint64_t a_desc = kWeight ? umma_desc_mn_sw128(a_addr, kChunk) : umma_desc_sw128(a_addr);
                     const uint64_t b_desc = umma_desc_mn_sw128(a_addr + 2 * kChunk, kChunk);
                     // 16 elements of the contraction on: 32 bytes of a K-major row, or two 1024-byte atoms
                     constexpr uint32_t kStepA = kWeight ? 2048 >> 4 : 32 >> 4, kStepB = 2048 >> 4;
+                    if (elect_one()) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        umma_bf16<2>(d_tmem, a_desc + kStepA * j, b_desc + kStepB * j, idesc, (st | j) != 0 ? 1u : 0u);
-                    umma_commit_2cta(empty(s), 3);
-                }
-                if (alive) umma_commit_2cta(tm_full(buf), 3);
-            }
-        } else if (lane == 0) {
-            uint32_t it = 0;
-            bool alive = true;
-            for (int tile = worker; alive && tile < num_tiles; tile += workers) {
-                for (int st = 0; st < steps; ++st, ++it) {
-                    const uint32_t s = it % S, r = it / S;
-                    if (!mbar_wait(full(s), r & 1u, abort_flag)) { alive = false; break; }
-                    mbar_arrive_cluster(peer_full(s), 0);
+                        for (int j = 0; j < 4; ++j)
+                            umma_bf16<2>(d_tmem, a_desc + kStepA * j, b_desc + kStepB * j, idesc, (st | j) != 0 ? 1u : 0u);
+                        umma_commit_2cta(empty(s), 3);
+                        if (st == steps - 1) umma_commit_2cta(tm_full(buf), 3);
+                    }
+                    __syncwarp();
                 }
             }
         }
