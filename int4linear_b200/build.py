@@ -19,7 +19,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libint4linear_b200.so")
 SOURCES = ["api.cu", "gemm_tcgen05.cu", "gemm_tcgen05_s8.cu", "gemm_skinny.cu", "gemm_legacy.cu", "packer.cu", "probe.cu", "gemm_fewrows.cu", "no_alloc.cu",
-           "api_fp4.cu", "fp4_quant.cu", "gemm_fp4.cu", "gemm_grad.cu"]
+           "api_fp4.cu", "fp4_quant.cu", "gemm_fp4.cu", "gemm_fp4_fewrows.cu", "gemm_grad.cu"]
 
 
 def _deps() -> list[str]:

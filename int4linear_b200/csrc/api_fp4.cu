@@ -44,6 +44,12 @@ int take_operands(const int4_linear_fp4_matrix* x, const int4_linear_fp4_matrix*
 
 bool bad_act(int act) { return act != INT4L_ACT_SILU && act != INT4L_ACT_GELU && act != INT4L_ACT_GELU_TANH; }
 
+int launch_product(DeviceCtx* ctx, const Fp4Problem& p, cudaStream_t stream)
+{
+    const bool few = fp4_fewrows_supports(p) && (p.m <= 64);
+    return few ? launch_fp4_fewrows(ctx, p, stream) : launch_fp4_gemm(ctx, p, stream);
+}
+
 // Pieces of a backward pass's workspace, in order, each on a 256-byte boundary.
 struct GradLayout {
     long long d0 = 0, d1 = 0, w0 = 0, w1 = 0, x = 0, bytes = 0, ld = 0;
@@ -107,7 +113,7 @@ int int4_linear_fp4_launch_async(const int4_linear_fp4_matrix* x, const int4_lin
     p.bias = bias_d;
     p.y = y_d;
     p.fp16 = y_type == INT4L_TYPE_F16;
-    return record_status(launch_fp4_gemm(ctx, p, static_cast<cudaStream_t>(stream)));
+    return record_status(launch_product(ctx, p, static_cast<cudaStream_t>(stream)));
 }
 
 int int4_linear_fp4_gated_launch_async(const int4_linear_fp4_matrix* x, const int4_linear_fp4_matrix* w_gate,
@@ -127,7 +133,7 @@ int int4_linear_fp4_gated_launch_async(const int4_linear_fp4_matrix* x, const in
     p.keep_gate = gate_d;
     p.keep_up = up_d;
     p.fp16 = h_type == INT4L_TYPE_F16;
-    return record_status(launch_fp4_gemm(ctx, p, static_cast<cudaStream_t>(stream)));
+    return record_status(launch_product(ctx, p, static_cast<cudaStream_t>(stream)));
 }
 
 long long int4_linear_fp4_grad_workspace_bytes(int m, int n, int k, int gated, int want_dx, int want_dw)

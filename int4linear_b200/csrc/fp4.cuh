@@ -76,5 +76,9 @@ int launch_gate_backward(DeviceCtx* ctx, const void* dh, const void* gate, const
                          const float* f_g, const float* f_u, int m, int n, long long ld, cudaStream_t stream);
 int setup_fp4_gemm(DeviceCtx* ctx);
 int launch_fp4_gemm(DeviceCtx* ctx, const Fp4Problem& p, cudaStream_t stream);
+// Few rows of x (gemm_fp4_fewrows.cu).
+int setup_fp4_fewrows(DeviceCtx* ctx);
+bool fp4_fewrows_supports(const Fp4Problem& p);
+int launch_fp4_fewrows(DeviceCtx* ctx, const Fp4Problem& p, cudaStream_t stream);
 
 }  // namespace i4l

@@ -64,14 +64,17 @@ class Fp4Matrix:
     128 rows x 4 scales (512 bytes, scale (r, j) at byte (r % 32) * 16 + (r // 32) * 4 + j), along k first, rows
     padded to 128 and scales to 4 (the padding along k must not be NaN; 0 is right).  `from_rows` builds it from
     scales in row order, `scale_rows` gives them back.  tensor_scale: nvfp4 only, float32 CUDA tensor of one
-    element or None (1).  The tensors are held, not copied: the matrix changes with them."""
+    element or None (1).  The tensors are held, not copied: the matrix changes with their values (their memory must stay
+    theirs: no resize_ or set_)."""
     codes: "torch.Tensor"  # noqa: F821
     scales: "torch.Tensor"  # noqa: F821
     rows: int
     k: int
     format: str = "mxfp4"
     tensor_scale: "torch.Tensor | None" = None  # noqa: F821
+    device: "torch.device" = field(init=False, repr=False)  # noqa: F821
     _c: _CMatrix = field(init=False, repr=False)
+    _p: int = field(init=False, repr=False)  # address of _c
 
     def __post_init__(self):
         import torch
@@ -90,13 +93,25 @@ class Fp4Matrix:
 
     def _wrap(self):
         ts = self.tensor_scale
-        object.__setattr__(self, "_c", _CMatrix(self.codes.data_ptr(), self.scales.data_ptr(),
-                                                ts.data_ptr() if ts is not None else None,
-                                                self.rows, self.k, FORMATS[self.format]))
+        d = self.__dict__  # (frozen for users; this is part of the construction)
+        d["device"] = self.codes.device
+        d["_c"] = c = _CMatrix(self.codes.data_ptr(), self.scales.data_ptr(), ts.data_ptr() if ts is not None else None,
+                               self.rows, self.k, FORMATS[self.format])
+        d["_p"] = ctypes.addressof(c)
 
-    @property
-    def device(self):
-        return self.codes.device
+    @classmethod
+    def _new(cls, rows: int, k: int, fmt: str, tensor_scale, device) -> "Fp4Matrix":
+        """An uninitialised matrix, its arguments already checked."""
+        import torch
+        q = object.__new__(cls)
+        q.__dict__.update(codes=torch.empty((rows, k // 2), dtype=torch.uint8, device=device),
+                          scales=torch.empty(_scale_bytes(rows, k, fmt), dtype=torch.uint8, device=device),
+                          rows=rows, k=k, format=fmt, tensor_scale=tensor_scale)
+        q._wrap()
+        return q
+
+    def __reduce__(self):  # copies and pickles are built anew: _c holds addresses
+        return type(self), (self.codes, self.scales, self.rows, self.k, self.format, self.tensor_scale)
 
     @property
     def shape(self):
@@ -125,39 +140,35 @@ class Fp4Matrix:
         return full[:self.rows, :blocks].contiguous()
 
 
-class _On:
-    """Device and stream of one call: makes them current (allocations included) where they are not."""
-    __slots__ = ("handle", "device", "ctx")
+def _where(device, stream, inputs):
+    """(stream handle, context to work in or None) of one call.  The context makes the device and stream current, so
+    that allocations belong to them; none is needed where they already are."""
+    import torch
+    if stream is None:
+        index = device.index
+        handle = torch._C._cuda_getCurrentRawStream(index)
+        return handle, None if torch.cuda.current_device() == index else torch.cuda.device(device)
+    if not hasattr(stream, "cuda_stream"):
+        stream = torch.cuda.ExternalStream(int(stream), device=device)
+    if stream.device != device:
+        raise ValueError("stream belongs to another device than the operands")
+    current = torch.cuda.current_stream(device)
+    if stream != current:
+        for t in inputs():  # their memory must not be handed out again before this stream is done with it
+            if t is not None:
+                t.record_stream(stream)
+    elif torch.cuda.current_device() == device.index:
+        return stream.cuda_stream, None
+    return stream.cuda_stream, torch.cuda.stream(stream)
 
-    def __init__(self, device, stream, inputs=()):
-        import torch
-        current = torch.cuda.current_stream(device)
-        self.ctx = None
-        if stream is None:
-            stream = current
-            if torch.cuda.current_device() != device.index:
-                self.ctx = torch.cuda.device(device)
-        else:
-            if not hasattr(stream, "cuda_stream"):
-                stream = torch.cuda.ExternalStream(int(stream), device=device)
-            if stream.device != device:
-                raise ValueError("stream belongs to another device than the operands")
-            if stream != current or torch.cuda.current_device() != device.index:
-                self.ctx = torch.cuda.stream(stream)
-            if stream != current:
-                for t in inputs:  # their memory must not be handed out again before this stream is done with it
-                    if t is not None:
-                        t.record_stream(stream)
-        self.handle = stream.cuda_stream
 
-    def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
-        return self.handle
-
-    def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
+def _run(body, device, stream, inputs):
+    """body(handle) on the call's device and stream."""
+    handle, ctx = _where(device, stream, inputs)
+    if ctx is None:
+        return body(handle)
+    with ctx:
+        return body(handle)
 
 
 def _type_of(dtype) -> int:
@@ -189,61 +200,74 @@ def quantize_fp4(x, format: str = "mxfp4", tensor_scale=None, out: Fp4Matrix | N
     scale = amax / 6 rounded to e4m3 per 16 elements.  Codes are rounded to nearest, ties to even, and saturate
     at 6.  A block that holds a NaN or an infinity becomes NaN.  `out`: a matrix of that shape and format to write
     into; its own tensor_scale is then used."""
-    import torch
     if not x.is_cuda or x.dim() != 2:
         raise ValueError("quantize_fp4 expects a 2-D CUDA tensor; there is no CPU implementation")
     rows, k = x.shape
+    device = x.device
     t = _type_of(x.dtype)
     if out is not None:
-        if out.shape != (rows, k) or out.device != x.device or tensor_scale is not None:
+        if out.shape != (rows, k) or out.device != device or tensor_scale is not None:
             raise ValueError("out must have the shape and device of x, and brings its own tensor_scale")
-        format, tensor_scale = out.format, out.tensor_scale
-    _check_shape(rows, k, format)
-    _check_tensor_scale(tensor_scale, format, x.device)
-    with _On(x.device, stream, (x, tensor_scale) if out is None else (x, *_parts(out))) as handle:
-        if x.stride(1) != 1 or (rows > 1 and x.stride(0) < k):
-            x = x.contiguous()
-        if out is None:
-            out = Fp4Matrix(torch.empty((rows, k // 2), dtype=torch.uint8, device=x.device),
-                            torch.empty(_scale_bytes(rows, k, format), dtype=torch.uint8, device=x.device),
-                            rows, k, format, tensor_scale)
+    else:
+        _check_shape(rows, k, format)
+        if tensor_scale is not None:
+            _check_tensor_scale(tensor_scale, format, device)
+
+    def body(handle):
+        src = x
+        pitch = x.stride(0) if rows > 1 else k
+        if x.stride(1) != 1 or pitch < k:
+            src, pitch = x.contiguous(), k
+        q = out if out is not None else Fp4Matrix._new(rows, k, format, tensor_scale, device)
         if rows:
-            pitch = x.stride(0) if rows > 1 else k
-            _check(_lib.load().int4_linear_fp4_quantize_async(x.data_ptr(), t, pitch, ctypes.byref(out._c), handle),
-                   "int4_linear_fp4_quantize_async")
-    return out
+            _check(_lib.load().int4_linear_fp4_quantize_async(src.data_ptr(), t, pitch, q._p, handle), "int4_linear_fp4_quantize_async")
+        return q
+
+    return _run(body, device, stream, lambda: (x, tensor_scale) if out is None else (x, *_parts(out)))
 
 
 def dequantize_fp4(q: Fp4Matrix, dtype=None, out=None, stream=None):
     """The values of a quantised matrix, [rows, k] float32 (or `dtype`: bfloat16, float16)."""
     import torch
-    dtype = dtype or (out.dtype if out is not None else torch.float32)
+    if dtype is None:
+        dtype = out.dtype if out is not None else torch.float32
     t = _type_of(dtype)
-    with _On(q.device, stream, (*_parts(q), out)) as handle:
-        if out is None:
-            out = torch.empty(q.shape, dtype=dtype, device=q.device)
-        else:
-            _check_out(out, q.shape, dtype, q.device)
+    if out is not None:
+        _check_out(out, q.shape, dtype, q.device)
+
+    def body(handle):
+        y = out if out is not None else torch.empty((q.rows, q.k), dtype=dtype, device=q.device)
         if q.rows:
-            _check(_lib.load().int4_linear_fp4_dequantize_async(ctypes.byref(q._c), out.data_ptr(), t, handle),
-                   "int4_linear_fp4_dequantize_async")
-    return out
+            _check(_lib.load().int4_linear_fp4_dequantize_async(q._p, y.data_ptr(), t, handle), "int4_linear_fp4_dequantize_async")
+        return y
+
+    return _run(body, q.device, stream, lambda: (*_parts(q), out))
 
 
 def _check_operands(x: Fp4Matrix, *ws: Fp4Matrix) -> tuple[int, int]:
+    rows = ws[0].rows
     for w in ws:
-        if w.k != x.k or w.format != x.format or w.device != x.device or w.rows != ws[0].rows:
+        if w.k != x.k or w.format != x.format or w.device != x.device or w.rows != rows:
             raise ValueError("operands must agree in k, format and device (and both weights in their rows)")
-    return x.rows, ws[0].rows
+    return x.rows, rows
 
 
 def _half(dtype, out):
+    """(output type, its INT4L_TYPE_ number)"""
     import torch
     if dtype is None:
         dtype = out.dtype if out is not None else torch.bfloat16
-    if dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError("the output is bfloat16 or float16")
-    return dtype
+    if dtype is torch.bfloat16:
+        return dtype, 0
+    if dtype is torch.float16:
+        return dtype, 1
+    raise ValueError("the output is bfloat16 or float16")
+
+
+def _check_act(activation: str) -> int:
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"unknown activation {activation!r}: expected one of {sorted(ACTIVATIONS)}")
+    return ACTIVATIONS[activation]
 
 
 def linear_fp4(x: Fp4Matrix, w: Fp4Matrix, bias=None, out=None, dtype=None, stream=None):
@@ -251,19 +275,20 @@ def linear_fp4(x: Fp4Matrix, w: Fp4Matrix, bias=None, out=None, dtype=None, stre
     `bias`: float32 CUDA vector of n elements."""
     import torch
     m, n = _check_operands(x, w)
-    dtype = _half(dtype, out)
+    dtype, t = _half(dtype, out)
     if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (n,) or bias.device != x.device or not bias.is_contiguous()):
         raise ValueError(f"bias must be a contiguous float32 tensor with {n} elements on the operands' device")
-    with _On(x.device, stream, (*_parts(x, w), bias, out)) as handle:
-        if out is None:
-            out = torch.empty((m, n), dtype=dtype, device=x.device)
-        else:
-            _check_out(out, (m, n), dtype, x.device)
+    if out is not None:
+        _check_out(out, (m, n), dtype, x.device)
+
+    def body(handle):
+        y = out if out is not None else torch.empty((m, n), dtype=dtype, device=x.device)
         if m and n:
-            _check(_lib.load().int4_linear_fp4_launch_async(
-                ctypes.byref(x._c), ctypes.byref(w._c), bias.data_ptr() if bias is not None else None, out.data_ptr(),
-                0 if dtype == torch.bfloat16 else 1, handle), "int4_linear_fp4_launch_async")
-    return out
+            _check(_lib.load().int4_linear_fp4_launch_async(x._p, w._p, bias.data_ptr() if bias is not None else None, y.data_ptr(),
+                                                            t, handle), "int4_linear_fp4_launch_async")
+        return y
+
+    return _run(body, x.device, stream, lambda: (*_parts(x, w), bias, out))
 
 
 def gated_linear_fp4(x: Fp4Matrix, w_gate: Fp4Matrix, w_up: Fp4Matrix, activation: str = "silu", out=None, dtype=None,
@@ -274,23 +299,21 @@ def gated_linear_fp4(x: Fp4Matrix, w_gate: Fp4Matrix, w_up: Fp4Matrix, activatio
     (H, gate, up), the products rounded to the same type, as gated_linear_fp4_backward takes them."""
     import torch
     m, n = _check_operands(x, w_gate, w_up)
-    dtype = _half(dtype, out)
-    if activation not in ACTIVATIONS:
-        raise ValueError(f"unknown activation {activation!r}: expected one of {sorted(ACTIVATIONS)}")
-    gate = up = None
-    with _On(x.device, stream, (*_parts(x, w_gate, w_up), out)) as handle:
-        if out is None:
-            out = torch.empty((m, n), dtype=dtype, device=x.device)
-        else:
-            _check_out(out, (m, n), dtype, x.device)
-        if save:
-            gate, up = torch.empty_like(out), torch.empty_like(out)
+    dtype, t = _half(dtype, out)
+    act = _check_act(activation)
+    if out is not None:
+        _check_out(out, (m, n), dtype, x.device)
+
+    def body(handle):
+        h = out if out is not None else torch.empty((m, n), dtype=dtype, device=x.device)
+        gate, up = (torch.empty_like(h), torch.empty_like(h)) if save else (None, None)
         if m and n:
             _check(_lib.load().int4_linear_fp4_gated_launch_async(
-                ctypes.byref(x._c), ctypes.byref(w_gate._c), ctypes.byref(w_up._c), ACTIVATIONS[activation], out.data_ptr(),
-                gate.data_ptr() if save else None, up.data_ptr() if save else None, 0 if dtype == torch.bfloat16 else 1, handle),
-                "int4_linear_fp4_gated_launch_async")
-    return (out, gate, up) if save else out
+                x._p, w_gate._p, w_up._p, act, h.data_ptr(), gate.data_ptr() if save else None, up.data_ptr() if save else None,
+                t, handle), "int4_linear_fp4_gated_launch_async")
+        return (h, gate, up) if save else h
+
+    return _run(body, x.device, stream, lambda: (*_parts(x, w_gate, w_up), out))
 
 
 def _check_grad(t, m: int, n: int, device, name: str):
@@ -312,20 +335,23 @@ def linear_fp4_backward(grad_y, x: Fp4Matrix, w: Fp4Matrix, need=(True, True), s
     m, n = _check_operands(x, w)
     _check_grad(grad_y, m, n, x.device, "grad_y")
     want_x, want_w = bool(need[0]), bool(need[1])
-    with _On(x.device, stream, (grad_y, *_parts(x, w))) as handle:
+
+    def body(handle):
         empty = m == 0 or n == 0  # an empty sum is 0
         new = torch.zeros if empty else torch.empty
         dx = new((m, x.k), dtype=torch.bfloat16, device=x.device) if want_x else None
         dw = new((n, x.k), dtype=torch.bfloat16, device=x.device) if want_w else None
         if not empty and (want_x or want_w):
-            grad_y = grad_y.contiguous()
-            if grad_y.data_ptr() % 16:
-                grad_y = grad_y.clone()
+            dy = grad_y.contiguous()
+            if dy.data_ptr() % 16:
+                dy = dy.clone()
             ws = _workspace(m, n, x.k, False, want_x, want_w, x.device)
             _check(_lib.load().int4_linear_fp4_grad_async(
-                grad_y.data_ptr(), ctypes.byref(x._c), ctypes.byref(w._c), dx.data_ptr() if want_x else None,
-                dw.data_ptr() if want_w else None, ws.data_ptr(), ws.numel(), handle), "int4_linear_fp4_grad_async")
-    return dx, dw
+                dy.data_ptr(), x._p, w._p, dx.data_ptr() if want_x else None, dw.data_ptr() if want_w else None,
+                ws.data_ptr(), ws.numel(), handle), "int4_linear_fp4_grad_async")
+        return dx, dw
+
+    return _run(body, x.device, stream, lambda: (grad_y, *_parts(x, w)))
 
 
 def gated_linear_fp4_backward(grad_h, gate, up, x: Fp4Matrix, w_gate: Fp4Matrix, w_up: Fp4Matrix, activation: str = "silu",
@@ -337,23 +363,24 @@ def gated_linear_fp4_backward(grad_h, gate, up, x: Fp4Matrix, w_gate: Fp4Matrix,
     `need` = (input, weights) leaves gradients out (None in their place)."""
     import torch
     m, n = _check_operands(x, w_gate, w_up)
-    if activation not in ACTIVATIONS:
-        raise ValueError(f"unknown activation {activation!r}: expected one of {sorted(ACTIVATIONS)}")
+    act = _check_act(activation)
     for t, name in ((grad_h, "grad_h"), (gate, "gate"), (up, "up")):
         _check_grad(t, m, n, x.device, name)
     want_x, want_w = bool(need[0]), bool(need[1])
-    with _On(x.device, stream, (grad_h, gate, up, *_parts(x, w_gate, w_up))) as handle:
+
+    def body(handle):
         empty = m == 0 or n == 0
         new = torch.zeros if empty else torch.empty
         dx = new((m, x.k), dtype=torch.bfloat16, device=x.device) if want_x else None
         dwg = new((n, x.k), dtype=torch.bfloat16, device=x.device) if want_w else None
         dwu = new((n, x.k), dtype=torch.bfloat16, device=x.device) if want_w else None
         if not empty and (want_x or want_w):
-            grad_h, gate, up = grad_h.contiguous(), gate.contiguous(), up.contiguous()
+            dh, g, u = grad_h.contiguous(), gate.contiguous(), up.contiguous()
             ws = _workspace(m, n, x.k, True, want_x, want_w, x.device)
             _check(_lib.load().int4_linear_fp4_gated_grad_async(
-                grad_h.data_ptr(), gate.data_ptr(), up.data_ptr(), ctypes.byref(x._c), ctypes.byref(w_gate._c),
-                ctypes.byref(w_up._c), ACTIVATIONS[activation], dx.data_ptr() if want_x else None,
+                dh.data_ptr(), g.data_ptr(), u.data_ptr(), x._p, w_gate._p, w_up._p, act, dx.data_ptr() if want_x else None,
                 dwg.data_ptr() if want_w else None, dwu.data_ptr() if want_w else None, ws.data_ptr(), ws.numel(), handle),
                 "int4_linear_fp4_gated_grad_async")
-    return dx, dwg, dwu
+        return dx, dwg, dwu
+
+    return _run(body, x.device, stream, lambda: (grad_h, gate, up, *_parts(x, w_gate, w_up)))
