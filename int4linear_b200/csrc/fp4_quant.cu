@@ -11,6 +11,7 @@
 // A block that holds a NaN or an infinity gets the scale NaN, and so does every product with it.
 //
 // Bound: HBM.  Each element is read once (2 or 4 bytes) and written once (half a byte and 1/32 or 1/16).
+#include "epilogue.cuh"
 #include "fp4.cuh"
 
 namespace i4l {
@@ -18,33 +19,12 @@ namespace i4l {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4;  // row chunks in flight per warp
+constexpr int kUnroll = 4;  // rows of a unit
 
 template <int kType> struct Src;
 template <> struct Src<INT4L_TYPE_BF16> { using T = __nv_bfloat16; };
 template <> struct Src<INT4L_TYPE_F16> { using T = __half; };
 template <> struct Src<INT4L_TYPE_F32> { using T = float; };
-
-__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_float(float v) { return v; }
-
-// Eight elements from p (any alignment; `vec` says 16 bytes).
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool vec, float (&v)[8])
-{
-    __align__(16) T e[8];
-    if (vec) {
-        constexpr int kVecs = sizeof(T) * 8 / 16;
-#pragma unroll
-        for (int i = 0; i < kVecs; ++i) reinterpret_cast<uint4*>(e)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = p[i];
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_float(e[i]);
-}
 
 // Eight floats -> eight codes, element 0 in the low nibble; nearest, ties to even, saturating.
 __device__ __forceinline__ uint32_t to_e2m1x8(const float (&v)[8])
@@ -76,10 +56,61 @@ __device__ __forceinline__ float from_e4m3(uint32_t byte)
     return __half2float(__ushort_as_half(static_cast<unsigned short>(h2 & 0xFFFFu)));
 }
 
-// One warp handles 256 consecutive elements of a row at a time, eight per lane: a lane's loads are 16 (or 32)
-// bytes, the warp's code store 128, and a block's scale is agreed on by 4 (mxfp4) or 2 (nvfp4) lanes.  The
-// words of a scale tile (4 scales) are put together by 16 or 8 lanes and stored by the first of them.
-// Rows are padded to 128 and scales to whole words with zeros, so that nothing in a scale tile is undefined.
+// Eight source elements and the largest magnitude among them as float bits (infinities and NaNs on top).
+template <typename T> struct Eight;
+template <> struct Eight<float> {
+    float v[8];
+    __device__ __forceinline__ float get(int e) const { return v[e]; }
+    __device__ __forceinline__ uint32_t top() const
+    {
+        uint32_t t = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t = max(t, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+        return t;
+    }
+};
+template <> struct Eight<__nv_bfloat16> {
+    uint32_t w[4];
+    __device__ __forceinline__ float get(int e) const { return __uint_as_float((e & 1) ? w[e / 2] & 0xFFFF0000u : w[e / 2] << 16); }
+    __device__ __forceinline__ uint32_t top() const
+    {
+        auto mag = [&](int i) { const uint32_t a = w[i] & 0x7FFF7FFFu; return *reinterpret_cast<const __nv_bfloat162*>(&a); };
+        const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(mag(0), mag(1)), __hmax2_nan(mag(2), mag(3)));
+        const uint32_t b = *reinterpret_cast<const uint32_t*>(&m);
+        return max(b << 16, b & 0xFFFF0000u);
+    }
+};
+template <> struct Eight<__half> {
+    uint32_t w[4];
+    __device__ __forceinline__ float get(int e) const
+    {
+        return __half2float(__ushort_as_half(static_cast<unsigned short>((e & 1) ? w[e / 2] >> 16 : w[e / 2] & 0xFFFFu)));
+    }
+    __device__ __forceinline__ uint32_t top() const
+    {
+        auto mag = [&](int i) { const uint32_t a = w[i] & 0x7FFF7FFFu; return *reinterpret_cast<const __half2*>(&a); };
+        const __half2 m = __hmax2_nan(__hmax2_nan(mag(0), mag(1)), __hmax2_nan(mag(2), mag(3)));
+        return max(__float_as_uint(__low2float(m)) & 0x7FFFFFFFu, __float_as_uint(__high2float(m)) & 0x7FFFFFFFu);
+    }
+};
+
+// A warp's unit: 256 consecutive elements (eight per lane) of four consecutive rows.  Both kernels were first bound by
+// instructions, most of them addresses: with a row of its own per step they took 143 (mxfp4), 236 (nvfp4) and 116
+// (expansion) instructions for eight elements; a unit's rows share the address arithmetic.
+struct Unit {
+    int row0, col;
+    __device__ __forceinline__ explicit Unit(int k)
+    {
+        const uint32_t u = blockIdx.x * (kThreads / 32) + threadIdx.x / 32, chunks = (k + 255u) / 256u;
+        const uint32_t group = u / chunks;
+        row0 = static_cast<int>(group * kUnroll);
+        col = static_cast<int>((u - group * chunks) * 256 + (threadIdx.x & 31) * 8);
+    }
+};
+
+// A lane's loads are 16 (or 32) bytes, the warp's code store 128, and a block's scale is agreed on by 4 (mxfp4) or 2
+// (nvfp4) lanes, whose first writes the byte.  Rows are padded to 128 and scales to whole words with zeros, so that
+// nothing in a scale tile is undefined.
 template <int kType, bool kBlock16>
 __global__ void __launch_bounds__(kThreads)
 fp4_quantize_kernel(const typename Src<kType>::T* __restrict__ src, long long pitch, uint8_t* __restrict__ codes,
@@ -87,187 +118,184 @@ fp4_quantize_kernel(const typename Src<kType>::T* __restrict__ src, long long pi
 {
     constexpr int kLanes = kBlock16 ? 2 : 4;  // lanes of a block
     using T = typename Src<kType>::T;
-    const int lane = threadIdx.x & 31;
-    const int chunks = (k + 255) / 256;
-    const int rows_padded = (rows + 127) / 128 * 128;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const Unit u(k);
+    if (u.row0 >= (rows + 127) / 128 * 128) return;  // (uniform over the warp)
     const int ktiles = fp4_ktiles(k, kBlock16);
-    const long long total = static_cast<long long>(rows_padded) * chunks;
-    const long long warps = static_cast<long long>(gridDim.x) * (kThreads / 32);
-    const bool vec = (reinterpret_cast<uintptr_t>(src) & 15u) == 0 && (pitch * sizeof(T)) % 16 == 0;
+    const bool in_k = u.col < k;
+    Eight<T> v[kUnroll];
+    {
+        const T* p = src + u.row0 * pitch + u.col;
+        const bool vec = ((reinterpret_cast<uintptr_t>(src) | (static_cast<uintptr_t>(pitch) * sizeof(T))) & 15u) == 0;
+#pragma unroll
+        for (int i = 0; i < kUnroll; ++i, p += pitch) {
+            v[i] = Eight<T>{};
+            if (!in_k || u.row0 + i >= rows) continue;
+            if (vec) {
+#pragma unroll
+                for (int q = 0; q < static_cast<int>(sizeof(v[i]) / 16); ++q) reinterpret_cast<uint4*>(&v[i])[q] = __ldg(reinterpret_cast<const uint4*>(p) + q);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) reinterpret_cast<T*>(&v[i])[e] = p[e];
+            }
+        }
+    }
     float inv = 1.0f;
     if (kBlock16 && tensor_scale != nullptr) {
         const float ts = __ldg(tensor_scale);
         inv = ts != 0.0f ? 1.0f / ts : 0.0f;
     }
-    for (long long u0 = (blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x) / 32; u0 < total; u0 += warps * kUnroll) {
-        float v[kUnroll][8];
-        int row[kUnroll], col[kUnroll];
+    const int block = u.col / (8 * kLanes);
+    uint8_t* scale_at = scales + fp4_scale_word(u.row0, block >> 2, ktiles) + (block & 3);  // row0 % 4 == 0: the next rows' are 16 bytes on
+    const bool writes_scale = (threadIdx.x & (kLanes - 1)) == 0 && block < 4 * ktiles;
+    uint8_t* code_at = codes + (static_cast<size_t>(u.row0) * k + u.col) / 2;
 #pragma unroll
-        for (int i = 0; i < kUnroll; ++i) {
-            const long long u = u0 + i * warps;
-            row[i] = u < total ? static_cast<int>(u / chunks) : rows_padded;
-            col[i] = static_cast<int>(u - static_cast<long long>(u / chunks) * chunks) * 256 + lane * 8;
-            if (row[i] < rows && col[i] < k) {
-                load8(src + row[i] * pitch + col[i], vec, v[i]);
-            } else {
+    for (int i = 0; i < kUnroll; ++i, code_at += k / 2) {
+        const bool live = in_k && u.row0 + i < rows;
+        uint32_t top = v[i].top();
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[i][e] = 0.0f;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < kUnroll; ++i) {
-            if (row[i] >= rows_padded) break;  // (uniform over the warp)
-            const bool live = row[i] < rows && col[i] < k;
-            uint32_t top = 0;  // |x| as bits: orders like the values, infinities and NaNs on top
+        for (int d = 1; d < kLanes; d *= 2) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+        uint32_t byte;
+        float x[8];
+        if constexpr (kBlock16) {
+            // Rounding is monotonic: the largest product is the product of the largest.
+            top = __float_as_uint(__uint_as_float(top) * inv) & 0x7FFFFFFFu;
+            // amax / 6, rounded to odd: with its last bit set where it is not exact, and on the exact quotient's side
+            // of every float with a trailing zero bit.  (The product errs by at most 1.5 ulp, and the quotients
+            // next to a tie between two e4m3 values lie at least 2/3 ulp from it, so stepping back once is enough.)
+            // 24 such bits round to e4m3's 4 as the exact quotient does.
+            const float a = __uint_as_float(top);
+            const float q = a * (1.0f / 6.0f);
+            const float rest = fmaf(-q, 6.0f, a);
+            uint32_t odd = __float_as_uint(q) - (rest < 0.0f ? 1u : 0u);
+            if (rest != 0.0f) odd |= 1u;
+            byte = to_e4m3(__uint_as_float(odd));
+            const float s = from_e4m3(byte);
+            // x / s: a quotient from the approximate reciprocal and one residual step (Markstein, "Computation of
+            // elementary functions on the IBM RISC System/6000", 1990).  A tie between two codes times s has at most
+            // 7 bits, so it is itself a float, whose quotient comes out exact; the quotients of its neighbours lie
+            // at least 1/1.875 = 0.53 ulp from the tie and are not rounded onto it.
+            const float r = s > 0.0f ? __fdividef(1.0f, s) : 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                if (kBlock16) v[i][e] *= inv;
-                top = max(top, __float_as_uint(v[i][e]) & 0x7FFFFFFFu);
+                const float t = v[i].get(e) * inv;
+                const float q0 = t * r;
+                x[e] = copysignf(fmaf(fmaf(-q0, s, t), r, q0), t);  // (the residual step loses the sign of -0)
             }
+            if (top >= 0x7F800000u) byte = 0x7Fu;
+        } else {
+            const int e8 = max(static_cast<int>(top >> 23) - 2, 0);
+            byte = static_cast<uint32_t>(e8);
+            // 2^(127 - e8), from 2^127 down to 2^-125: exact, and normal wherever a value survives
+            const float r = __uint_as_float(static_cast<uint32_t>(254 - e8) << 23);
 #pragma unroll
-            for (int d = 1; d < kLanes; d *= 2) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-            uint32_t byte;
-            if constexpr (kBlock16) {
-                // amax / 6 cut short with its last bit set when anything was lost (round to odd): 24 such bits
-                // round to e4m3's 4 as the exact quotient does.
-                const float a = __uint_as_float(top);
-                float q = __fdiv_rz(a, 6.0f);
-                if (fmaf(-q, 6.0f, a) != 0.0f) q = __uint_as_float(__float_as_uint(q) | 1u);
-                byte = to_e4m3(q);
-                const float s = from_e4m3(byte);
-                // x / s correctly rounded from a correctly rounded reciprocal and one residual step
-                // (Markstein, "Computation of elementary functions on the IBM RISC System/6000", 1990).  No
-                // rounding of it lands on a tie that the exact quotient misses: a tie times s has at most 7 bits,
-                // so it is itself a float, and the quotients of its neighbours are at least an ulp away.
-                const float r = s > 0.0f ? __frcp_rn(s) : 0.0f;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float q0 = v[i][e] * r;
-                    v[i][e] = copysignf(fmaf(fmaf(-q0, s, v[i][e]), r, q0), v[i][e]);  // (the residual step loses the sign of -0)
-                }
-                if (top >= 0x7F800000u) byte = 0x7Fu;
-            } else {
-                const int e8 = max(static_cast<int>(top >> 23) - 2, 0);
-                byte = static_cast<uint32_t>(e8);
-                // 2^(127 - e8), from 2^127 down to 2^-125: exact, and normal wherever a value survives
-                const float r = __uint_as_float(static_cast<uint32_t>(254 - e8) << 23);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[i][e] *= r;
-                if (top >= 0x7F800000u) byte = 0xFFu;
-            }
-            if (!live) byte = 0;
-            if (live) reinterpret_cast<uint32_t*>(codes)[(static_cast<size_t>(row[i]) * k + col[i]) / 8] = to_e2m1x8(v[i]);
-            // Four neighbouring scales -> one word.
-            uint32_t word = byte;
-            word |= __shfl_down_sync(0xFFFFFFFFu, byte, kLanes) << 8;
-            word |= __shfl_down_sync(0xFFFFFFFFu, byte, 2 * kLanes) << 16;
-            word |= __shfl_down_sync(0xFFFFFFFFu, byte, 3 * kLanes) << 24;
-            const int kt = col[i] / (4 * kLanes * 8);
-            if (lane % (4 * kLanes) == 0 && kt < ktiles)
-                *reinterpret_cast<uint32_t*>(scales + fp4_scale_word(row[i], kt, ktiles)) = word;
+            for (int e = 0; e < 8; ++e) x[e] = v[i].get(e) * r;
+            if (top >= 0x7F800000u) byte = 0xFFu;
         }
+        if (live) *reinterpret_cast<uint32_t*>(code_at) = to_e2m1x8(x);
+        if (writes_scale) scale_at[16 * i] = static_cast<uint8_t>(live ? byte : 0);
     }
 }
 
-// Eight codes and their scale -> eight values per thread.
+// The same units: eight codes and their scale -> eight values per lane and row.
 template <int kType, bool kBlock16>
 __global__ void __launch_bounds__(kThreads)
 fp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, const float* __restrict__ tensor_scale,
                       int apply_tensor_scale, typename Src<kType>::T* __restrict__ dst, int rows, int k)
 {
     using T = typename Src<kType>::T;
-    const int words = k / 8;
-    const int ktiles = fp4_ktiles(k, kBlock16);
-    const long long total = static_cast<long long>(rows) * words;
-    const long long stride = static_cast<long long>(gridDim.x) * kThreads;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const Unit u(k);
+    if (u.row0 >= rows || u.col >= k) return;
+    const int block = u.col / (kBlock16 ? 16 : 32);
+    const uint8_t* scale_at = scales + fp4_scale_word(u.row0, block >> 2, fp4_ktiles(k, kBlock16)) + (block & 3);
+    const size_t first = static_cast<size_t>(u.row0) * k + u.col;
+    uint32_t word[kUnroll], byte[kUnroll];
+    {
+        const uint8_t* p = codes + first / 2;
+#pragma unroll
+        for (int i = 0; i < kUnroll; ++i, p += k / 2) {
+            if (u.row0 + i >= rows) break;
+            word[i] = __ldg(reinterpret_cast<const uint32_t*>(p));
+            byte[i] = __ldg(scale_at + 16 * i);
+        }
+    }
     float ts = tensor_scale != nullptr ? __ldg(tensor_scale) : 1.0f;
     // Operands of the gradient products keep the tensor scale out (their epilogue applies it), but a matrix
     // whose tensor scale is 0 is 0 there too.
     if (!apply_tensor_scale) ts = ts == 0.0f ? 0.0f : 1.0f;
-    for (long long i0 = blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x; i0 < total; i0 += stride * kUnroll) {
-        uint32_t word[kUnroll];
-        uint32_t byte[kUnroll];
+    T* d = dst + first;
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const long long i = i0 + u * stride;
-            if (i < total) {
-                const int row = static_cast<int>(i / words), col = static_cast<int>(i - static_cast<long long>(row) * words) * 8;
-                const int blk = col / (kBlock16 ? 16 : 32);
-                word[u] = __ldg(reinterpret_cast<const uint32_t*>(codes) + i);
-                byte[u] = __ldg(scales + fp4_scale_word(row, blk >> 2, ktiles) + (blk & 3));
-            }
+    for (int i = 0; i < kUnroll; ++i, d += k) {
+        if (u.row0 + i >= rows) break;
+        float s;
+        if constexpr (kBlock16) {
+            s = from_e4m3(byte[i]);  // 0x7F converts to NaN
+        } else {
+            // 2^(b - 127); 2^-127 is subnormal
+            s = byte[i] == 0xFFu ? __uint_as_float(0x7FFFFFFFu) : __uint_as_float(byte[i] ? byte[i] << 23 : 0x00400000u);
+        }
+        const bool scaled = kBlock16 && ts != 1.0f;
+        uint32_t h2[4];  // the codes as eight halves
+        asm("{\n\t"
+            ".reg .b8 c0, c1, c2, c3;\n\t"
+            "mov.b32 {c0, c1, c2, c3}, %4;\n\t"
+            "cvt.rn.f16x2.e2m1x2 %0, c0;\n\t"
+            "cvt.rn.f16x2.e2m1x2 %1, c1;\n\t"
+            "cvt.rn.f16x2.e2m1x2 %2, c2;\n\t"
+            "cvt.rn.f16x2.e2m1x2 %3, c3;\n\t"
+            "}\n" : "=r"(h2[0]), "=r"(h2[1]), "=r"(h2[2]), "=r"(h2[3]) : "r"(word[i]));
+        __align__(16) T out[8];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const float2 c = __half22float2(*reinterpret_cast<const __half2*>(&h2[b]));
+            float lo = c.x * s, hi = c.y * s;  // exact
+            if (scaled) { lo *= ts; hi *= ts; }
+            if constexpr (kType == INT4L_TYPE_BF16) reinterpret_cast<uint32_t*>(out)[b] = pack16<false>(lo, hi);
+            else if constexpr (kType == INT4L_TYPE_F16) reinterpret_cast<uint32_t*>(out)[b] = pack16<true>(lo, hi);
+            else { out[2 * b] = lo; out[2 * b + 1] = hi; }
         }
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const long long i = i0 + u * stride;
-            if (i >= total) break;
-            float s;
-            if constexpr (kBlock16) {
-                s = from_e4m3(byte[u]);  // 0x7F converts to NaN
-            } else {
-                // 2^(b - 127); 2^-127 is subnormal
-                s = byte[u] == 0xFFu ? __uint_as_float(0x7FFFFFFFu) : __uint_as_float(byte[u] ? byte[u] << 23 : 0x00400000u);
-            }
-            __align__(16) T out[8];
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                uint32_t h2;
-                asm("{\n\t.reg .b8 c;\n\tcvt.u8.u32 c, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, c;\n\t}\n" : "=r"(h2) : "r"((word[u] >> (8 * b)) & 0xFFu));
-                const float lo = __half2float(__ushort_as_half(static_cast<unsigned short>(h2 & 0xFFFFu)));
-                const float hi = __half2float(__ushort_as_half(static_cast<unsigned short>(h2 >> 16)));
-                if constexpr (kType == INT4L_TYPE_BF16) {
-                    out[2 * b] = __float2bfloat16_rn(lo * s * ts);
-                    out[2 * b + 1] = __float2bfloat16_rn(hi * s * ts);
-                } else if constexpr (kType == INT4L_TYPE_F16) {
-                    out[2 * b] = __float2half_rn(lo * s * ts);
-                    out[2 * b + 1] = __float2half_rn(hi * s * ts);
-                } else {
-                    out[2 * b] = lo * s * ts;
-                    out[2 * b + 1] = hi * s * ts;
-                }
-            }
-            uint4* d = reinterpret_cast<uint4*>(dst + i * 8);
-#pragma unroll
-            for (int q = 0; q < static_cast<int>(sizeof(T)) / 2; ++q) d[q] = reinterpret_cast<const uint4*>(out)[q];
-        }
+        for (int q = 0; q < static_cast<int>(sizeof(T)) / 2; ++q) reinterpret_cast<uint4*>(d)[q] = reinterpret_cast<const uint4*>(out)[q];
     }
 }
 
-// Enough blocks to fill the GPU a few times over, fewer when there is less to do.
-int grid_for(const DeviceCtx* ctx, long long units_per_block_pass, long long units)
+template <typename... P, typename... A>
+int launch_units(DeviceCtx* ctx, void (*kernel)(P...), long long rows, int k, cudaStream_t stream, A... args)
 {
-    const long long want = (units + units_per_block_pass - 1) / units_per_block_pass;
-    const long long cap = static_cast<long long>(ctx->sm_count) * 16;
-    return static_cast<int>(want < 1 ? 1 : (want < cap ? want : cap));
+    const long long units = rows / kUnroll * ((k + 255) / 256), blocks = (units + kThreads / 32 - 1) / (kThreads / 32);
+    if (blocks > 0x1FFFFFFF) return INT4L_ERR_TOO_LARGE;  // (units are counted in 32 bits; 4 T elements)
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(blocks), 1, 1);
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    count_launch();
+    if (e != cudaSuccess) { cudaGetLastError(); return INT4L_ERR_CUDA; }
+    return INT4L_OK;
 }
 
 template <int kType>
 int quantize_typed(DeviceCtx* ctx, const void* src, long long pitch, const Fp4& d, cudaStream_t stream)
 {
     using T = typename Src<kType>::T;
-    const long long units = static_cast<long long>((d.rows + 127ll) / 128 * 128) * ((d.k + 255) / 256);
-    const int grid = grid_for(ctx, kThreads / 32, units);
-    uint8_t* codes = const_cast<uint8_t*>(d.codes);
-    uint8_t* scales = const_cast<uint8_t*>(d.scales);
-    if (d.block16)
-        fp4_quantize_kernel<kType, true><<<grid, kThreads, 0, stream>>>(static_cast<const T*>(src), pitch, codes, scales, d.tensor_scale, d.rows, d.k);
-    else
-        fp4_quantize_kernel<kType, false><<<grid, kThreads, 0, stream>>>(static_cast<const T*>(src), pitch, codes, scales, d.tensor_scale, d.rows, d.k);
-    count_launch();
-    return cudaGetLastError() == cudaSuccess ? INT4L_OK : INT4L_ERR_CUDA;
+    return launch_units(ctx, d.block16 ? fp4_quantize_kernel<kType, true> : fp4_quantize_kernel<kType, false>, (d.rows + 127ll) / 128 * 128, d.k, stream,
+                        static_cast<const T*>(src), pitch, const_cast<uint8_t*>(d.codes), const_cast<uint8_t*>(d.scales), d.tensor_scale, d.rows, d.k);
 }
 
 template <int kType>
 int dequantize_typed(DeviceCtx* ctx, const Fp4& s, void* dst, bool apply, cudaStream_t stream)
 {
     using T = typename Src<kType>::T;
-    const int grid = grid_for(ctx, kThreads * kUnroll, static_cast<long long>(s.rows) * (s.k / 8));
-    if (s.block16)
-        fp4_dequantize_kernel<kType, true><<<grid, kThreads, 0, stream>>>(s.codes, s.scales, s.tensor_scale, apply, static_cast<T*>(dst), s.rows, s.k);
-    else
-        fp4_dequantize_kernel<kType, false><<<grid, kThreads, 0, stream>>>(s.codes, s.scales, s.tensor_scale, apply, static_cast<T*>(dst), s.rows, s.k);
-    count_launch();
-    return cudaGetLastError() == cudaSuccess ? INT4L_OK : INT4L_ERR_CUDA;
+    return launch_units(ctx, s.block16 ? fp4_dequantize_kernel<kType, true> : fp4_dequantize_kernel<kType, false>, (s.rows + 3ll) / 4 * 4, s.k, stream,
+                        s.codes, s.scales, s.tensor_scale, static_cast<int>(apply), static_cast<T*>(dst), s.rows, s.k);
 }
 
 }  // namespace
