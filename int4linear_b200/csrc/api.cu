@@ -205,7 +205,7 @@ DeviceCtx* current_ctx(int* status)
     if (rc == INT4L_OK) rc = setup_fewrows(c);
     if (rc == INT4L_OK) rc = setup_fp4_gemm(c);
     if (rc == INT4L_OK) rc = setup_fp4_fewrows(c);
-    if (rc == INT4L_OK) rc = setup_grad(c);
+    if (rc == INT4L_OK) rc = setup_fp4_backward(c);
     if (rc != INT4L_OK) { *status = rc; return nullptr; }
     c->attrs_set = true;
     g_ctx_ready[dev] = true;

@@ -50,20 +50,18 @@ int launch_product(DeviceCtx* ctx, const Fp4Problem& p, cudaStream_t stream)
     return few ? launch_fp4_fewrows(ctx, p, stream) : launch_fp4_gemm(ctx, p, stream);
 }
 
-// Pieces of a backward pass's workspace, in order, each on a 256-byte boundary.
-struct GradLayout {
-    long long d0 = 0, d1 = 0, w0 = 0, w1 = 0, x = 0, bytes = 0, ld = 0;
-};
-GradLayout grad_layout(long long m, long long n, long long k, bool gated, bool want_dx, bool want_dw)
+// The common part of both backward passes.
+int run_backward(Fp4Backward& b, void* workspace_d, long long workspace_bytes, void* stream)
 {
-    GradLayout l;
-    l.ld = (n + 7) / 8 * 8;
-    auto piece = [&](long long bytes) { const long long at = l.bytes; l.bytes += (bytes + 255) / 256 * 256; return at; };
-    if (gated) { l.d0 = piece(m * l.ld * 2); l.d1 = piece(m * l.ld * 2); }
-    else if (n % 8 != 0) l.d0 = piece(m * l.ld * 2);
-    if (want_dx) { l.w0 = piece(n * k * 2); if (gated) l.w1 = piece(n * k * 2); }
-    if (want_dw) l.x = piece(m * k * 2);
-    return l;
+    const Fp4Problem& p = b.forward;
+    if (!b.dx && !b.dw) return INT4L_ERR_INVALID_ARG;
+    if (misaligned(b.dx, 16) || misaligned(b.dw, 16) || misaligned(b.dw_up, 16) || misaligned(workspace_d, 256)) return INT4L_ERR_MISALIGNED;
+    if (!workspace_d || workspace_bytes < fp4_backward_workspace(p.m, p.n, p.k, p.gated, b.dx != nullptr, b.dw != nullptr)) return INT4L_ERR_INVALID_ARG;
+    int rc = INT4L_OK;
+    DeviceCtx* ctx = current_ctx(&rc);
+    if (!ctx) return rc;
+    b.workspace = static_cast<uint8_t*>(workspace_d);
+    return launch_fp4_backward(ctx, b, static_cast<cudaStream_t>(stream));
 }
 
 }  // namespace
@@ -96,7 +94,7 @@ int int4_linear_fp4_dequantize_async(const int4_linear_fp4_matrix* src, void* ds
     if (rc == INT4L_OK && misaligned(dst_d, 16)) rc = INT4L_ERR_MISALIGNED;
     if (rc != INT4L_OK) return record_status(rc);
     DeviceCtx* ctx = current_ctx(&rc);
-    if (ctx) rc = launch_fp4_dequantize(ctx, s, dst_d, dst_type, true, static_cast<cudaStream_t>(stream));
+    if (ctx) rc = launch_fp4_dequantize(ctx, s, dst_d, dst_type, static_cast<cudaStream_t>(stream));
     return record_status(rc);
 }
 
@@ -139,51 +137,21 @@ int int4_linear_fp4_gated_launch_async(const int4_linear_fp4_matrix* x, const in
 long long int4_linear_fp4_grad_workspace_bytes(int m, int n, int k, int gated, int want_dx, int want_dw)
 {
     if (m <= 0 || n <= 0 || k <= 0) return -INT4L_ERR_INVALID_ARG;
-    return grad_layout(m, n, k, gated != 0, want_dx != 0, want_dw != 0).bytes;
+    return fp4_backward_workspace(m, n, k, gated != 0, want_dx != 0, want_dw != 0);
 }
 
 int int4_linear_fp4_grad_async(const void* dy_d, const int4_linear_fp4_matrix* x, const int4_linear_fp4_matrix* w,
                                void* dx_d, void* dw_d, void* workspace_d, long long workspace_bytes, void* stream)
 {
-    Fp4Problem p;
-    int rc = take_operands(x, w, nullptr, false, &p);
-    if (rc == INT4L_OK && (!dy_d || (!dx_d && !dw_d))) rc = INT4L_ERR_INVALID_ARG;
-    if (rc == INT4L_OK && (misaligned(dy_d, 16) || misaligned(dx_d, 16) || misaligned(dw_d, 16) || misaligned(workspace_d, 256))) rc = INT4L_ERR_MISALIGNED;
+    Fp4Backward b;
+    int rc = take_operands(x, w, nullptr, false, &b.forward);
+    if (rc == INT4L_OK && !dy_d) rc = INT4L_ERR_INVALID_ARG;
+    if (rc == INT4L_OK && misaligned(dy_d, b.forward.n % 8 == 0 ? 16 : 2)) rc = INT4L_ERR_MISALIGNED;
     if (rc != INT4L_OK) return record_status(rc);
-    const GradLayout l = grad_layout(p.m, p.n, p.k, false, dx_d != nullptr, dw_d != nullptr);
-    if (!workspace_d || workspace_bytes < l.bytes) return record_status(INT4L_ERR_INVALID_ARG);
-    DeviceCtx* ctx = current_ctx(&rc);
-    if (!ctx) return record_status(rc);
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    uint8_t* ws = static_cast<uint8_t*>(workspace_d);
-    GradProduct g;
-    g.m = p.m; g.n = p.n; g.k = p.k; g.ld = l.ld;
-    g.d0 = dy_d;
-    if (p.n % 8 != 0) {  // TMA needs a 16-byte row pitch
-        if (cudaMemcpy2DAsync(ws + l.d0, l.ld * 2, dy_d, p.n * 2ull, p.n * 2ull, p.m, cudaMemcpyDeviceToDevice, s) != cudaSuccess) {
-            cudaGetLastError();
-            return record_status(INT4L_ERR_CUDA);
-        }
-        g.d0 = ws + l.d0;
-    }
-    if (rc == INT4L_OK && dx_d) {
-        rc = launch_fp4_dequantize(ctx, p.w, ws + l.w0, INT4L_TYPE_BF16, false, s);
-        GradProduct d = g;
-        d.b0 = ws + l.w0;
-        d.out = dx_d;
-        d.num = p.w.tensor_scale;
-        if (rc == INT4L_OK) rc = launch_grad_product(ctx, d, s);
-    }
-    if (rc == INT4L_OK && dw_d) {
-        rc = launch_fp4_dequantize(ctx, p.x, ws + l.x, INT4L_TYPE_BF16, false, s);
-        GradProduct d = g;
-        d.weight = true;
-        d.b0 = ws + l.x;
-        d.out = dw_d;
-        d.num = p.x.tensor_scale;
-        if (rc == INT4L_OK) rc = launch_grad_product(ctx, d, s);
-    }
-    return record_status(rc);
+    b.dy = dy_d;
+    b.dx = dx_d;
+    b.dw = dw_d;
+    return record_status(run_backward(b, workspace_d, workspace_bytes, stream));
 }
 
 int int4_linear_fp4_gated_grad_async(const void* dh_d, const void* gate_d, const void* up_d, const int4_linear_fp4_matrix* x,
@@ -191,48 +159,19 @@ int int4_linear_fp4_gated_grad_async(const void* dh_d, const void* gate_d, const
                                      void* dx_d, void* dw_gate_d, void* dw_up_d, void* workspace_d, long long workspace_bytes,
                                      void* stream)
 {
-    Fp4Problem p;
-    int rc = take_operands(x, w_gate, w_up, true, &p);
-    if (rc == INT4L_OK && (!dh_d || !gate_d || !up_d || (!dx_d && !dw_gate_d) || !dw_gate_d != !dw_up_d || bad_act(activation))) rc = INT4L_ERR_INVALID_ARG;
-    if (rc == INT4L_OK && (misaligned(dh_d, 2) || misaligned(gate_d, 2) || misaligned(up_d, 2) || misaligned(dx_d, 16) ||
-                           misaligned(dw_gate_d, 16) || misaligned(dw_up_d, 16) || misaligned(workspace_d, 256)))
-        rc = INT4L_ERR_MISALIGNED;
+    Fp4Backward b;
+    int rc = take_operands(x, w_gate, w_up, true, &b.forward);
+    if (rc == INT4L_OK && (!dh_d || !gate_d || !up_d || !dw_gate_d != !dw_up_d || bad_act(activation))) rc = INT4L_ERR_INVALID_ARG;
+    if (rc == INT4L_OK && (misaligned(dh_d, 2) || misaligned(gate_d, 2) || misaligned(up_d, 2))) rc = INT4L_ERR_MISALIGNED;
     if (rc != INT4L_OK) return record_status(rc);
-    const GradLayout l = grad_layout(p.m, p.n, p.k, true, dx_d != nullptr, dw_gate_d != nullptr);
-    if (!workspace_d || workspace_bytes < l.bytes) return record_status(INT4L_ERR_INVALID_ARG);
-    DeviceCtx* ctx = current_ctx(&rc);
-    if (!ctx) return record_status(rc);
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    uint8_t* ws = static_cast<uint8_t*>(workspace_d);
-    // dg and du carry their weight's tensor scale, so that dx is one contraction over both; the weight
-    // gradients take it out again.
-    rc = launch_gate_backward(ctx, dh_d, gate_d, up_d, ws + l.d0, ws + l.d1, activation, p.w.tensor_scale, p.w_up.tensor_scale,
-                              p.m, p.n, l.ld, s);
-    GradProduct g;
-    g.m = p.m; g.n = p.n; g.k = p.k; g.ld = l.ld;
-    if (rc == INT4L_OK && dx_d) {
-        rc = launch_fp4_dequantize(ctx, p.w, ws + l.w0, INT4L_TYPE_BF16, false, s);
-        if (rc == INT4L_OK) rc = launch_fp4_dequantize(ctx, p.w_up, ws + l.w1, INT4L_TYPE_BF16, false, s);
-        GradProduct d = g;
-        d.d0 = ws + l.d0; d.d1 = ws + l.d1;
-        d.b0 = ws + l.w0; d.b1 = ws + l.w1;
-        d.out = dx_d;
-        if (rc == INT4L_OK) rc = launch_grad_product(ctx, d, s);
-    }
-    if (rc == INT4L_OK && dw_gate_d) {
-        rc = launch_fp4_dequantize(ctx, p.x, ws + l.x, INT4L_TYPE_BF16, false, s);
-        for (int i = 0; i < 2 && rc == INT4L_OK; ++i) {
-            GradProduct d = g;
-            d.weight = true;
-            d.d0 = ws + (i ? l.d1 : l.d0);
-            d.b0 = ws + l.x;
-            d.out = i ? dw_up_d : dw_gate_d;
-            d.num = p.x.tensor_scale;
-            d.den = i ? p.w_up.tensor_scale : p.w.tensor_scale;
-            rc = launch_grad_product(ctx, d, s);
-        }
-    }
-    return record_status(rc);
+    b.forward.act = activation;
+    b.dy = dh_d;
+    b.gate = gate_d;
+    b.up = up_d;
+    b.dx = dx_d;
+    b.dw = dw_gate_d;
+    b.dw_up = dw_up_d;
+    return record_status(run_backward(b, workspace_d, workspace_bytes, stream));
 }
 
 }  // extern "C"

@@ -54,26 +54,21 @@ struct Fp4Problem {
 };
 
 int launch_fp4_quantize(DeviceCtx* ctx, const void* src, int src_type, long long src_pitch, const Fp4& dst, cudaStream_t stream);
-int launch_fp4_dequantize(DeviceCtx* ctx, const Fp4& src, void* dst, int dst_type, bool apply_tensor_scale, cudaStream_t stream);
-// The gradient products (gemm_grad.cu), bf16 operands and result, fp32 accumulation; alpha = num / den, a null
-// pointer or a 0 in den counting as 1.
-//     input gradient    dx[m x k] = alpha (d0[m x n] w0[n x k] + d1 w1)    (d1 / w1 null: one product)
-//     weight gradient   dw[n x k] = alpha d0[m x n]^T x[m x k]
-// d0 / d1 have a row pitch of `ld` elements (a multiple of 8).
-struct GradProduct {
-    bool weight = false;
-    const void* d0 = nullptr; const void* d1 = nullptr;
-    const void* b0 = nullptr; const void* b1 = nullptr;  // w0, w1, or x
-    void* out = nullptr;
-    int m = 0, n = 0, k = 0;
-    long long ld = 0;
-    const float* num = nullptr; const float* den = nullptr;
+int launch_fp4_dequantize(DeviceCtx* ctx, const Fp4& src, void* dst, int dst_type, cudaStream_t stream);
+// Backward pass of a product or a gated product (gemm_grad.cu); x, w, w_up and m, n, k as in `forward`.
+struct Fp4Backward {
+    Fp4Problem forward;
+    const void* dy = nullptr;             // m x n bf16: the gradient of y or h
+    const void* gate = nullptr;           // gated: the kept products
+    const void* up = nullptr;
+    void* dx = nullptr;                   // m x k, or null
+    void* dw = nullptr;                   // n x k, or null (gated: the gate's, and dw_up with it)
+    void* dw_up = nullptr;
+    uint8_t* workspace = nullptr;         // fp4_backward_workspace() bytes, 256-byte aligned
 };
-int setup_grad(DeviceCtx* ctx);
-int launch_grad_product(DeviceCtx* ctx, const GradProduct& p, cudaStream_t stream);
-// dg = dh u act'(g) f_g, du = dh act(g) f_u as bf16 with row pitch ld; f = the tensor scale of that weight (0 counts as 1).
-int launch_gate_backward(DeviceCtx* ctx, const void* dh, const void* gate, const void* up, void* dg, void* du, int act,
-                         const float* f_g, const float* f_u, int m, int n, long long ld, cudaStream_t stream);
+long long fp4_backward_workspace(long long m, long long n, long long k, bool gated, bool want_dx, bool want_dw);
+int setup_fp4_backward(DeviceCtx* ctx);
+int launch_fp4_backward(DeviceCtx* ctx, const Fp4Backward& b, cudaStream_t stream);
 int setup_fp4_gemm(DeviceCtx* ctx);
 int launch_fp4_gemm(DeviceCtx* ctx, const Fp4Problem& p, cudaStream_t stream);
 // Few rows of x (gemm_fp4_fewrows.cu).

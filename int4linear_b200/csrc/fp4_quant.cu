@@ -11,20 +11,11 @@
 // A block that holds a NaN or an infinity gets the scale NaN, and so does every product with it.
 //
 // Bound: HBM.  Each element is read once (2 or 4 bytes) and written once (half a byte and 1/32 or 1/16).
-#include "epilogue.cuh"
-#include "fp4.cuh"
+#include "fp4_expand.cuh"
 
 namespace i4l {
 
 namespace {
-
-constexpr int kThreads = 256;
-constexpr int kUnroll = 4;  // rows of a unit
-
-template <int kType> struct Src;
-template <> struct Src<INT4L_TYPE_BF16> { using T = __nv_bfloat16; };
-template <> struct Src<INT4L_TYPE_F16> { using T = __half; };
-template <> struct Src<INT4L_TYPE_F32> { using T = float; };
 
 // Eight floats -> eight codes, element 0 in the low nibble; nearest, ties to even, saturating.
 __device__ __forceinline__ uint32_t to_e2m1x8(const float (&v)[8])
@@ -49,13 +40,6 @@ __device__ __forceinline__ uint32_t to_e4m3(float a)
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.0f), "f"(a));
     return r & 0xFFu;
 }
-__device__ __forceinline__ float from_e4m3(uint32_t byte)
-{
-    uint32_t h2;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(static_cast<uint16_t>(byte)));
-    return __half2float(__ushort_as_half(static_cast<unsigned short>(h2 & 0xFFFFu)));
-}
-
 // Eight source elements and the largest magnitude among them as float bits (infinities and NaNs on top).
 template <typename T> struct Eight;
 template <> struct Eight<float> {
@@ -94,50 +78,41 @@ template <> struct Eight<__half> {
     }
 };
 
-// A warp's unit: 256 consecutive elements (eight per lane) of four consecutive rows.  Both kernels were first bound by
-// instructions, most of them addresses: with a row of its own per step they took 143 (mxfp4), 236 (nvfp4) and 116
-// (expansion) instructions for eight elements; a unit's rows share the address arithmetic.
-struct Unit {
-    int row0, col;
-    __device__ __forceinline__ explicit Unit(int k)
-    {
-        const uint32_t u = blockIdx.x * (kThreads / 32) + threadIdx.x / 32, chunks = (k + 255u) / 256u;
-        const uint32_t group = u / chunks;
-        row0 = static_cast<int>(group * kUnroll);
-        col = static_cast<int>((u - group * chunks) * 256 + (threadIdx.x & 31) * 8);
-    }
-};
-
-// A lane's loads are 16 (or 32) bytes, the warp's code store 128, and a block's scale is agreed on by 4 (mxfp4) or 2
-// (nvfp4) lanes, whose first writes the byte.  Rows are padded to 128 and scales to whole words with zeros, so that
+// kE elements per lane: 8, or 16, a whole nvfp4 block (its scale takes as many instructions as eight elements do).  A
+// block's scale is agreed on by its lanes, whose first writes the byte.  Rows are padded to 128 and scales to whole words with zeros, so that
 // nothing in a scale tile is undefined.
-template <int kType, bool kBlock16>
-__global__ void __launch_bounds__(kThreads)
+template <int kType, bool kBlock16, int kE>
+__global__ void __launch_bounds__(kUnitThreads)
 fp4_quantize_kernel(const typename Src<kType>::T* __restrict__ src, long long pitch, uint8_t* __restrict__ codes,
                     uint8_t* __restrict__ scales, const float* __restrict__ tensor_scale, int rows, int k)
 {
-    constexpr int kLanes = kBlock16 ? 2 : 4;  // lanes of a block
+    constexpr int kLanes = (kBlock16 ? 16 : 32) / kE;  // lanes of a block
+    constexpr int kH = kE / 8;
     using T = typename Src<kType>::T;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const Unit u(k);
+    const Unit<kE> u(blockIdx.x, k);
     if (u.row0 >= (rows + 127) / 128 * 128) return;  // (uniform over the warp)
     const int ktiles = fp4_ktiles(k, kBlock16);
     const bool in_k = u.col < k;
-    Eight<T> v[kUnroll];
+    Eight<T> v[kUnitRows][kH];
     {
         const T* p = src + u.row0 * pitch + u.col;
         const bool vec = ((reinterpret_cast<uintptr_t>(src) | (static_cast<uintptr_t>(pitch) * sizeof(T))) & 15u) == 0;
 #pragma unroll
-        for (int i = 0; i < kUnroll; ++i, p += pitch) {
-            v[i] = Eight<T>{};
-            if (!in_k || u.row0 + i >= rows) continue;
-            if (vec) {
+        for (int i = 0; i < kUnitRows; ++i, p += pitch) {
 #pragma unroll
-                for (int q = 0; q < static_cast<int>(sizeof(v[i]) / 16); ++q) reinterpret_cast<uint4*>(&v[i])[q] = __ldg(reinterpret_cast<const uint4*>(p) + q);
-            } else {
+            for (int h = 0; h < kH; ++h) {
+                v[i][h] = Eight<T>{};
+                if (!in_k || u.row0 + i >= rows) continue;
+                if (vec) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) reinterpret_cast<T*>(&v[i])[e] = p[e];
+                    for (int q = 0; q < static_cast<int>(sizeof(Eight<T>) / 16); ++q)
+                        reinterpret_cast<uint4*>(&v[i][h])[q] = __ldg(reinterpret_cast<const uint4*>(p + 8 * h) + q);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) reinterpret_cast<T*>(&v[i][h])[e] = p[8 * h + e];
+                }
             }
         }
     }
@@ -146,18 +121,19 @@ fp4_quantize_kernel(const typename Src<kType>::T* __restrict__ src, long long pi
         const float ts = __ldg(tensor_scale);
         inv = ts != 0.0f ? 1.0f / ts : 0.0f;
     }
-    const int block = u.col / (8 * kLanes);
+    const int block = u.col / (kE * kLanes);
     uint8_t* scale_at = scales + fp4_scale_word(u.row0, block >> 2, ktiles) + (block & 3);  // row0 % 4 == 0: the next rows' are 16 bytes on
     const bool writes_scale = (threadIdx.x & (kLanes - 1)) == 0 && block < 4 * ktiles;
     uint8_t* code_at = codes + (static_cast<size_t>(u.row0) * k + u.col) / 2;
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i, code_at += k / 2) {
+    for (int i = 0; i < kUnitRows; ++i, code_at += k / 2) {
         const bool live = in_k && u.row0 + i < rows;
-        uint32_t top = v[i].top();
+        uint32_t top = v[i][0].top();
+        if constexpr (kH == 2) top = max(top, v[i][1].top());
 #pragma unroll
         for (int d = 1; d < kLanes; d *= 2) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
         uint32_t byte;
-        float x[8];
+        float x[kH][8];
         if constexpr (kBlock16) {
             // Rounding is monotonic: the largest product is the product of the largest.
             top = __float_as_uint(__uint_as_float(top) * inv) & 0x7FFFFFFFu;
@@ -178,10 +154,10 @@ fp4_quantize_kernel(const typename Src<kType>::T* __restrict__ src, long long pi
             // at least 1/1.875 = 0.53 ulp from the tie and are not rounded onto it.
             const float r = s > 0.0f ? __fdividef(1.0f, s) : 0.0f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float t = v[i].get(e) * inv;
+            for (int e = 0; e < kE; ++e) {
+                const float t = v[i][e / 8].get(e & 7) * inv;
                 const float q0 = t * r;
-                x[e] = copysignf(fmaf(fmaf(-q0, s, t), r, q0), t);  // (the residual step loses the sign of -0)
+                x[e / 8][e & 7] = copysignf(fmaf(fmaf(-q0, s, t), r, q0), t);  // (the residual step loses the sign of -0)
             }
             if (top >= 0x7F800000u) byte = 0x7Fu;
         } else {
@@ -190,86 +166,35 @@ fp4_quantize_kernel(const typename Src<kType>::T* __restrict__ src, long long pi
             // 2^(127 - e8), from 2^127 down to 2^-125: exact, and normal wherever a value survives
             const float r = __uint_as_float(static_cast<uint32_t>(254 - e8) << 23);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = v[i].get(e) * r;
+            for (int e = 0; e < 8; ++e) x[0][e] = v[i][0].get(e) * r;
             if (top >= 0x7F800000u) byte = 0xFFu;
         }
-        if (live) *reinterpret_cast<uint32_t*>(code_at) = to_e2m1x8(x);
+        if (live) {
+            if constexpr (kH == 2) *reinterpret_cast<uint2*>(code_at) = make_uint2(to_e2m1x8(x[0]), to_e2m1x8(x[1]));
+            else *reinterpret_cast<uint32_t*>(code_at) = to_e2m1x8(x[0]);
+        }
         if (writes_scale) scale_at[16 * i] = static_cast<uint8_t>(live ? byte : 0);
     }
 }
 
-// The same units: eight codes and their scale -> eight values per lane and row.
 template <int kType, bool kBlock16>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kUnitThreads)
 fp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, const float* __restrict__ tensor_scale,
-                      int apply_tensor_scale, typename Src<kType>::T* __restrict__ dst, int rows, int k)
+                      typename Src<kType>::T* __restrict__ dst, int rows, int k)
 {
-    using T = typename Src<kType>::T;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const Unit u(k);
-    if (u.row0 >= rows || u.col >= k) return;
-    const int block = u.col / (kBlock16 ? 16 : 32);
-    const uint8_t* scale_at = scales + fp4_scale_word(u.row0, block >> 2, fp4_ktiles(k, kBlock16)) + (block & 3);
-    const size_t first = static_cast<size_t>(u.row0) * k + u.col;
-    uint32_t word[kUnroll], byte[kUnroll];
-    {
-        const uint8_t* p = codes + first / 2;
-#pragma unroll
-        for (int i = 0; i < kUnroll; ++i, p += k / 2) {
-            if (u.row0 + i >= rows) break;
-            word[i] = __ldg(reinterpret_cast<const uint32_t*>(p));
-            byte[i] = __ldg(scale_at + 16 * i);
-        }
-    }
-    float ts = tensor_scale != nullptr ? __ldg(tensor_scale) : 1.0f;
-    // Operands of the gradient products keep the tensor scale out (their epilogue applies it), but a matrix
-    // whose tensor scale is 0 is 0 there too.
-    if (!apply_tensor_scale) ts = ts == 0.0f ? 0.0f : 1.0f;
-    T* d = dst + first;
-#pragma unroll
-    for (int i = 0; i < kUnroll; ++i, d += k) {
-        if (u.row0 + i >= rows) break;
-        float s;
-        if constexpr (kBlock16) {
-            s = from_e4m3(byte[i]);  // 0x7F converts to NaN
-        } else {
-            // 2^(b - 127); 2^-127 is subnormal
-            s = byte[i] == 0xFFu ? __uint_as_float(0x7FFFFFFFu) : __uint_as_float(byte[i] ? byte[i] << 23 : 0x00400000u);
-        }
-        const bool scaled = kBlock16 && ts != 1.0f;
-        uint32_t h2[4];  // the codes as eight halves
-        asm("{\n\t"
-            ".reg .b8 c0, c1, c2, c3;\n\t"
-            "mov.b32 {c0, c1, c2, c3}, %4;\n\t"
-            "cvt.rn.f16x2.e2m1x2 %0, c0;\n\t"
-            "cvt.rn.f16x2.e2m1x2 %1, c1;\n\t"
-            "cvt.rn.f16x2.e2m1x2 %2, c2;\n\t"
-            "cvt.rn.f16x2.e2m1x2 %3, c3;\n\t"
-            "}\n" : "=r"(h2[0]), "=r"(h2[1]), "=r"(h2[2]), "=r"(h2[3]) : "r"(word[i]));
-        __align__(16) T out[8];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const float2 c = __half22float2(*reinterpret_cast<const __half2*>(&h2[b]));
-            float lo = c.x * s, hi = c.y * s;  // exact
-            if (scaled) { lo *= ts; hi *= ts; }
-            if constexpr (kType == INT4L_TYPE_BF16) reinterpret_cast<uint32_t*>(out)[b] = pack16<false>(lo, hi);
-            else if constexpr (kType == INT4L_TYPE_F16) reinterpret_cast<uint32_t*>(out)[b] = pack16<true>(lo, hi);
-            else { out[2 * b] = lo; out[2 * b + 1] = hi; }
-        }
-#pragma unroll
-        for (int q = 0; q < static_cast<int>(sizeof(T)) / 2; ++q) reinterpret_cast<uint4*>(d)[q] = reinterpret_cast<const uint4*>(out)[q];
-    }
+    fp4_expand_block<kType, kBlock16>(blockIdx.x, codes, scales, tensor_scale, true, dst, rows, k);
 }
 
 template <typename... P, typename... A>
-int launch_units(DeviceCtx* ctx, void (*kernel)(P...), long long rows, int k, cudaStream_t stream, A... args)
+int launch_units(DeviceCtx* ctx, void (*kernel)(P...), long long rows, int k, int elems, cudaStream_t stream, A... args)
 {
-    const long long units = rows / kUnroll * ((k + 255) / 256), blocks = (units + kThreads / 32 - 1) / (kThreads / 32);
+    const long long units = rows / kUnitRows * ((k + 32ll * elems - 1) / (32 * elems)), blocks = (units + kUnitThreads / 32 - 1) / (kUnitThreads / 32);
     if (blocks > 0x1FFFFFFF) return INT4L_ERR_TOO_LARGE;  // (units are counted in 32 bits; 4 T elements)
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(blocks), 1, 1);
-    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.blockDim = dim3(kUnitThreads, 1, 1);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -286,16 +211,24 @@ template <int kType>
 int quantize_typed(DeviceCtx* ctx, const void* src, long long pitch, const Fp4& d, cudaStream_t stream)
 {
     using T = typename Src<kType>::T;
-    return launch_units(ctx, d.block16 ? fp4_quantize_kernel<kType, true> : fp4_quantize_kernel<kType, false>, (d.rows + 127ll) / 128 * 128, d.k, stream,
-                        static_cast<const T*>(src), pitch, const_cast<uint8_t*>(d.codes), const_cast<uint8_t*>(d.scales), d.tensor_scale, d.rows, d.k);
+    const long long rows = (d.rows + 127ll) / 128 * 128;
+    auto launch = [&](auto kernel, int elems) {
+        return launch_units(ctx, kernel, rows, d.k, elems, stream, static_cast<const T*>(src), pitch, const_cast<uint8_t*>(d.codes),
+                            const_cast<uint8_t*>(d.scales), d.tensor_scale, d.rows, d.k);
+    };
+    if (!d.block16) return launch(fp4_quantize_kernel<kType, false, 8>, 8);
+    // 16 elements per lane take fewer instructions (8192 x 8192 bf16: 36.3 us against 41.1), 8 have the shorter way
+    // where the GPU is not filled anyway (16 x 4096: 2.1 us against 2.7).
+    return static_cast<long long>(d.rows) * d.k >= (1 << 20) ? launch(fp4_quantize_kernel<kType, true, 16>, 16)
+                                                             : launch(fp4_quantize_kernel<kType, true, 8>, 8);
 }
 
 template <int kType>
-int dequantize_typed(DeviceCtx* ctx, const Fp4& s, void* dst, bool apply, cudaStream_t stream)
+int dequantize_typed(DeviceCtx* ctx, const Fp4& s, void* dst, cudaStream_t stream)
 {
     using T = typename Src<kType>::T;
-    return launch_units(ctx, s.block16 ? fp4_dequantize_kernel<kType, true> : fp4_dequantize_kernel<kType, false>, (s.rows + 3ll) / 4 * 4, s.k, stream,
-                        s.codes, s.scales, s.tensor_scale, static_cast<int>(apply), static_cast<T*>(dst), s.rows, s.k);
+    return launch_units(ctx, s.block16 ? fp4_dequantize_kernel<kType, true> : fp4_dequantize_kernel<kType, false>, (s.rows + 3ll) / 4 * 4, s.k, 8, stream,
+                        s.codes, s.scales, s.tensor_scale, static_cast<T*>(dst), s.rows, s.k);
 }
 
 }  // namespace
@@ -309,12 +242,12 @@ int launch_fp4_quantize(DeviceCtx* ctx, const void* src, int src_type, long long
     }
 }
 
-int launch_fp4_dequantize(DeviceCtx* ctx, const Fp4& src, void* dst, int dst_type, bool apply_tensor_scale, cudaStream_t stream)
+int launch_fp4_dequantize(DeviceCtx* ctx, const Fp4& src, void* dst, int dst_type, cudaStream_t stream)
 {
     switch (dst_type) {
-        case INT4L_TYPE_BF16: return dequantize_typed<INT4L_TYPE_BF16>(ctx, src, dst, apply_tensor_scale, stream);
-        case INT4L_TYPE_F16: return dequantize_typed<INT4L_TYPE_F16>(ctx, src, dst, apply_tensor_scale, stream);
-        default: return dequantize_typed<INT4L_TYPE_F32>(ctx, src, dst, apply_tensor_scale, stream);
+        case INT4L_TYPE_BF16: return dequantize_typed<INT4L_TYPE_BF16>(ctx, src, dst, stream);
+        case INT4L_TYPE_F16: return dequantize_typed<INT4L_TYPE_F16>(ctx, src, dst, stream);
+        default: return dequantize_typed<INT4L_TYPE_F32>(ctx, src, dst, stream);
     }
 }
 

@@ -9,15 +9,24 @@
 // loses nothing (a code times its e8m0 or e4m3 scale has at most 6 significant bits); only the incoming gradient
 // is rounded, dg and du to bf16, as the gradients of a bf16 network are.
 //
-// The products are one persistent kernel, a CTA pair per 256 x 256 tile (tcgen05.mma kind::f16, cta_group::2),
-// two accumulators in tensor memory so that the epilogue overlaps the next tile:
+// Two launches.  The first prepares: dg and du (or dy with a row pitch that TMA takes), and the expansions.  The second
+// is all products in one persistent kernel, a CTA pair per 256 x 256 tile (tcgen05.mma kind::f16, cta_group::2), two
+// accumulators in tensor memory so that the epilogue overlaps the next tile:
 //     warp 0      TMA, steps of 64 along the contraction, into 128-byte-swizzled slots
 //     warp 1      UMMA issue (CTA 0 for both)
 //     warps 2-5   epilogue: scale, round to bf16, staged TMA stores
 // No operand is ever transposed: where the contraction runs down the rows of a matrix (w and x always, dy for
 // dw), its tile is read as it lies and the UMMA takes it MN-major.
+//
+// The tensor scales are kept out of the expanded matrices.  dx = dg wg + du wu is one contraction over both, so dg and
+// du are multiplied by their weight's tensor scale before they are rounded, and the weight gradients take it out again.
+//
+// dx and dw tiles have contractions of different length (n or 2 n, and m), and with separate launches each product
+// leaves a partly filled last wave.  Together they are dealt out in advance: the longer kind round-robin, the shorter
+// kind first to the workers that got one fewer, then round-robin (4096 x 14336 x 4096: 24 + 26 -> 49 of 46.5 waves of
+// the weight gradients' tile time).
 #include "epilogue.cuh"
-#include "fp4.cuh"
+#include "fp4_expand.cuh"
 #include "gate.cuh"
 #include "ptx.cuh"
 
@@ -25,29 +34,191 @@ namespace i4l {
 
 namespace {
 
+// ------------------------------------------------------------- preparation
+
+// dg = dh u act'(g) f_g, du = dh act(g) f_u with a row pitch of ld; without `gate` a copy of dh.
+struct GateJob {
+    const __nv_bfloat16* dh; const __nv_bfloat16* gate; const __nv_bfloat16* up;
+    __nv_bfloat16* dg; __nv_bfloat16* du;
+    const float* f_g; const float* f_u;
+    int m, n, act, vec;
+    long long ld;
+};
+struct ExpandJob {
+    const uint8_t* codes; const uint8_t* scales; const float* tensor_scale;
+    __nv_bfloat16* dst;
+    int rows, k;
+};
+// Blocks [0, first[0]) belong to the gate, [first[i], first[i + 1]) to expansion i.
+struct PrepArgs {
+    GateJob gate;
+    ExpandJob expand[3];
+    uint32_t first[4];
+};
+
+template <int kAct>
+__device__ __forceinline__ void gate_grad(float dh, float g, float u, float fg, float fu, float& dg, float& du)
+{
+    float act, slope;
+    gate_act_slope<kAct>(g, act, slope);
+    dg = dh * u * slope * fg;
+    du = dh * act * fu;
+}
+
+// A warp's unit: 256 columns of one row, eight per lane (consecutive where 16-byte accesses are possible, else 32
+// apart).  Bound by HBM: 10 bytes per element.
+template <int kAct>
+__device__ __forceinline__ void gate_block(const GateJob& j, uint32_t block)
+{
+    const uint32_t u = block * (kUnitThreads / 32) + threadIdx.x / 32, chunks = (j.n + 255u) / 256u;
+    const uint32_t row = u / chunks;
+    if (row >= static_cast<uint32_t>(j.m)) return;
+    const int lane = threadIdx.x & 31, col0 = (u - row * chunks) * 256;
+    const size_t src = static_cast<size_t>(row) * j.n, dst = static_cast<size_t>(row) * j.ld;
+    float fg = j.f_g != nullptr ? __ldg(j.f_g) : 1.0f, fu = j.f_u != nullptr ? __ldg(j.f_u) : 1.0f;
+    if (fg == 0.0f) fg = 1.0f;
+    if (fu == 0.0f) fu = 1.0f;
+    __align__(16) __nv_bfloat16 h[8] = {}, g[8] = {}, up[8] = {}, og[8], ou[8];
+    auto one = [&](int e) {
+        float a, b;
+        gate_grad<kAct>(__bfloat162float(h[e]), __bfloat162float(g[e]), __bfloat162float(up[e]), fg, fu, a, b);
+        og[e] = __float2bfloat16_rn(a);
+        ou[e] = __float2bfloat16_rn(b);
+    };
+    if (j.vec) {
+        const int col = col0 + lane * 8;
+        if (col >= j.n) return;
+        *reinterpret_cast<uint4*>(h) = __ldg(reinterpret_cast<const uint4*>(j.dh + src + col));
+        *reinterpret_cast<uint4*>(g) = __ldg(reinterpret_cast<const uint4*>(j.gate + src + col));
+        *reinterpret_cast<uint4*>(up) = __ldg(reinterpret_cast<const uint4*>(j.up + src + col));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) one(e);
+        *reinterpret_cast<uint4*>(j.dg + dst + col) = *reinterpret_cast<const uint4*>(og);
+        *reinterpret_cast<uint4*>(j.du + dst + col) = *reinterpret_cast<const uint4*>(ou);
+    } else {
+        const int col = col0 + lane;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (col + 32 * e < j.n) { h[e] = j.dh[src + col + 32 * e]; g[e] = j.gate[src + col + 32 * e]; up[e] = j.up[src + col + 32 * e]; }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (col + 32 * e < j.n) { one(e); j.dg[dst + col + 32 * e] = og[e]; j.du[dst + col + 32 * e] = ou[e]; }
+    }
+}
+
+__device__ __forceinline__ void copy_block(const GateJob& j, uint32_t block)
+{
+    const uint32_t u = block * (kUnitThreads / 32) + threadIdx.x / 32, chunks = (j.n + 255u) / 256u;
+    const uint32_t row = u / chunks;
+    if (row >= static_cast<uint32_t>(j.m)) return;
+    const int col = (u - row * chunks) * 256 + (threadIdx.x & 31);
+    const size_t src = static_cast<size_t>(row) * j.n, dst = static_cast<size_t>(row) * j.ld;
+    __nv_bfloat16 v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (col + 32 * e < j.n) v[e] = j.dh[src + col + 32 * e];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (col + 32 * e < j.n) j.dg[dst + col + 32 * e] = v[e];
+}
+
+template <bool kBlock16>
+__global__ void __launch_bounds__(kUnitThreads)
+backward_prepare_kernel(const __grid_constant__ PrepArgs a)
+{
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const uint32_t b = blockIdx.x;
+    if (b < a.first[0]) {
+        if (a.gate.gate == nullptr) copy_block(a.gate, b);
+        else if (a.gate.act == kActSilu) gate_block<kActSilu>(a.gate, b);
+        else if (a.gate.act == kActGelu) gate_block<kActGelu>(a.gate, b);
+        else gate_block<kActGeluTanh>(a.gate, b);
+    } else {
+        const int i = b < a.first[1] ? 0 : (b < a.first[2] ? 1 : 2);
+        const ExpandJob& j = a.expand[i];
+        fp4_expand_block<INT4L_TYPE_BF16, kBlock16>(b - a.first[i], j.codes, j.scales, j.tensor_scale, false, j.dst, j.rows, j.k);
+    }
+}
+
+// ---------------------------------------------------------------- products
+
 constexpr int kBM = 128, kBN = 256, kStepK = 64;
 constexpr int kThreads = 32 * 6;
 constexpr int kStages = 6;
 constexpr int kStage = 2 * 128 * 128;          // A and B tile of one CTA, 16 KB each
-constexpr int kChunk = kStepK * 128;           // MN-major: 64 columns x 64 rows
+constexpr int kChunk = kStepK * 128;           // a box: 64 columns x 64 rows
 constexpr int kStoreStage = 4096;              // per warp and buffer
 constexpr int kNumBarriers = 2 * kStages + 4;
 constexpr int kSmemBytes = 1024 + kStages * kStage + 4 * 2 * kStoreStage + kNumBarriers * 8 + 16;
 static_assert(kSmemBytes <= 232448, "shared memory budget");
 
+// One kind of tile: dx (its A operand is K-major), or a weight gradient (`matrices` of them, A MN-major).
+struct Kind {
+    int weight, matrices;
+    int rows, cols;         // of one result
+    int tiles_m, tiles_n;   // of one result
+    int steps;              // of a whole contraction
+};
 struct GradArgs {
-    const float* num; const float* den;
-    int rows, cols;        // of the result
-    int tiles_m, tiles_n;
-    int steps, segments;   // steps per segment of the contraction
+    Kind kind[2];           // the one with the longer contraction first; kind[1] may have no tiles
+    int tiles[2];
+    int segment;            // dx: steps of the first of its two contractions
+    int extra;              // tiles of kind 1 that a worker with one fewer of kind 0 takes first
+    const float* num; const float* den[2];  // dw[i] *= num / den[i]
+    const float* dx_scale;                  // dx *= this
     int* status;
 };
+struct Maps {
+    CUtensorMap d[2], w[2], x, dx, dw[2];
+};
 
-template <bool kWeight>
+// The i-th tile of a worker: its kind and index; false when there is none.
+__device__ __forceinline__ bool tile_of(const GradArgs& a, int worker, int workers, int i, int& kind, int& tile)
+{
+    const int mine = worker < a.tiles[0] ? (a.tiles[0] - worker + workers - 1) / workers : 0;
+    if (i < mine) { kind = 0; tile = worker + i * workers; return true; }
+    kind = 1;
+    i -= mine;
+    const int full = a.tiles[0] % workers;  // workers [full, workers) have one tile of kind 0 fewer
+    const int few = workers - full;
+    const int dealt = min(static_cast<long long>(few) * a.extra, static_cast<long long>(a.tiles[1]));
+    if (worker >= full) {
+        const int at = worker - full, own = at < dealt ? (dealt - at + few - 1) / few : 0;
+        if (i < own) { tile = at + i * few; return true; }
+        i -= own;
+    }
+    const long long t = dealt + worker + static_cast<long long>(i) * workers;
+    tile = static_cast<int>(t);
+    return t < a.tiles[1];
+}
+
+struct Tile {
+    const Kind* kind;
+    int weight, matrix, tm, tn;
+};
+__device__ __forceinline__ bool take_tile(const GradArgs& a, int worker, int workers, int i, Tile& t)
+{
+    int kind, tile;
+    if (!tile_of(a, worker, workers, i, kind, tile)) return false;
+    const Kind& k = a.kind[kind];
+    t.kind = &k;
+    t.weight = k.weight;
+    const int per = k.tiles_m * k.tiles_n;
+    t.matrix = tile / per;
+    tile -= t.matrix * per;
+    // Raster: groups of 16 row blocks share their column panel in L2.
+    constexpr int kGroupM = 16;
+    const int group = tile / (kGroupM * k.tiles_n);
+    const int gm = min(k.tiles_m - group * kGroupM, kGroupM);
+    const int in_group = tile - group * kGroupM * k.tiles_n;
+    t.tm = group * kGroupM + in_group % gm;
+    t.tn = in_group / gm;
+    return true;
+}
+
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-grad_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constant__ CUtensorMap tm_a1,
-                 const __grid_constant__ CUtensorMap tm_b0, const __grid_constant__ CUtensorMap tm_b1,
-                 const __grid_constant__ CUtensorMap tm_c, const __grid_constant__ GradArgs a)
+grad_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GradArgs a)
 {
     constexpr int S = kStages;
     extern __shared__ uint8_t smem_raw[];
@@ -58,10 +229,10 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
     const uint32_t ring = base;
     const uint32_t st_base = ring + S * kStage;
     const uint32_t bar_base = st_base + 4 * 2 * kStoreStage;
-    auto full     = [&](int i) { return bar_base + 8u * i; };
+    auto full     = [&](int i) { return bar_base + 8u * i; };  // (CTA 0's, for the loads of both)
     auto empty    = [&](int i) { return bar_base + 8u * (S + i); };
     auto tm_full  = [&](int i) { return bar_base + 8u * (2 * S + i); };
-    auto tm_empty  = [&](int i) { return bar_base + 8u * (2 * S + 2 + i); };
+    auto tm_empty = [&](int i) { return bar_base + 8u * (2 * S + 2 + i); };
     const uint32_t misc_off = (bar_base - base) + 8u * kNumBarriers;
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gbase + misc_off);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + misc_off + 4);
@@ -71,14 +242,12 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
     const int worker = static_cast<int>(cluster_id_x());
     const int workers = static_cast<int>(cluster_count_x());
 
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (tid == 0) {
         for (int i = 0; i < S; ++i) { mbar_init(full(i), 1); mbar_init(empty(i), 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(tm_full(i), 1); mbar_init(tm_empty(i), 4 * 2); }
         *abort_flag = 0;
         mbar_init_fence();
-        tma_prefetch_desc(&tm_a0);
-        tma_prefetch_desc(&tm_b0);
-        tma_prefetch_desc(&tm_c);
     }
     if (warp == 1) {
         tmem_alloc<2>(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
@@ -88,30 +257,17 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
     cluster_sync_all();
     tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot;
-
-    const int num_tiles = a.tiles_m * a.tiles_n;
-    const int steps = a.steps * a.segments;
-    constexpr int kGroupM = 16;
-    auto tile_coord = [&](int tile, int& tm, int& tn) {
-        const int group_size = kGroupM * a.tiles_n;
-        const int group = tile / group_size;
-        const int first_m = group * kGroupM;
-        const int gm = min(a.tiles_m - first_m, kGroupM);
-        const int in_group = tile - group * group_size;
-        tm = first_m + in_group % gm;
-        tn = in_group / gm;
-    };
+    asm volatile("griddepcontrol.wait;" ::: "memory");
 
     if (warp == 0) {
         // ------------------------------------------------------ TMA producer
         uint32_t it = 0;
         bool alive = true;
-        for (int tile = worker; alive && tile < num_tiles; tile += workers) {
-            int tm, tn;
-            tile_coord(tile, tm, tn);
-            const int row = (tm * 2 + static_cast<int>(cta_rank)) * kBM;
-            const int col = tn * kBN + static_cast<int>(cta_rank) * 128;
-            for (int st = 0; st < steps; ++st, ++it) {
+        Tile t;
+        for (int i = 0; alive && take_tile(a, worker, workers, i, t); ++i) {
+            const int row = (t.tm * 2 + static_cast<int>(cta_rank)) * kBM;
+            const int col = t.tn * kBN + static_cast<int>(cta_rank) * 128;
+            for (int st = 0; st < t.kind->steps; ++st, ++it) {
                 const uint32_t s = it % S, r = it / S;
                 if (!mbar_wait_warp(empty(s), (r & 1u) ^ 1u, abort_flag)) { alive = false; break; }
                 if (elect_one()) {
@@ -119,16 +275,13 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
                     if (cta_rank == 0) mbar_expect_tx(full(s), 2 * kStage);
                     const uint32_t bar = cluster_address(full(s), 0);
                     const uint32_t dst = ring + s * kStage;
-                    const bool second = st >= a.steps;
-                    const int k0 = (second ? st - a.steps : st) * kStepK;
-                    const CUtensorMap* ta = second ? &tm_a1 : &tm_a0;
-                    const CUtensorMap* tb = second ? &tm_b1 : &tm_b0;
-                    if constexpr (kWeight) {
-                        tma_load_2d_pair(dst, ta, bar, row, k0);
-                        tma_load_2d_pair(dst + kChunk, ta, bar, row + 64, k0);
-                    } else {
-                        tma_load_2d_pair(dst, ta, bar, k0, row);
-                    }
+                    // dx contracts over d[0], w[0] and then, for a gated product, d[1], w[1].
+                    const int part = t.weight ? t.matrix : (st >= a.segment ? 1 : 0);
+                    const int k0 = (t.weight || part == 0 ? st : st - a.segment) * kStepK;
+                    const CUtensorMap* ta = &maps.d[part];
+                    const CUtensorMap* tb = t.weight ? &maps.x : &maps.w[part];
+                    tma_load_2d_pair(dst, ta, bar, t.weight ? row : k0, t.weight ? k0 : row);
+                    tma_load_2d_pair(dst + kChunk, ta, bar, t.weight ? row + 64 : k0, t.weight ? k0 : row + 64);
                     tma_load_2d_pair(dst + 2 * kChunk, tb, bar, col, k0);
                     tma_load_2d_pair(dst + 3 * kChunk, tb, bar, col + 64, k0);
                 }
@@ -139,29 +292,30 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
         if (cta_rank == 0) {
             // ----------------------------------------------------- UMMA issuer
             // The warp walks the ring together and one elected thread issues.
-            constexpr uint32_t idesc = umma_idesc_bf16(2 * kBM, kBN, kWeight, true);
-            uint32_t it = 0, local_tile = 0;
+            uint32_t it = 0;
             bool alive = true;
-            for (int tile = worker; alive && tile < num_tiles; tile += workers, ++local_tile) {
-                const uint32_t buf = local_tile & 1u, br = local_tile >> 1;
+            Tile t;
+            for (int i = 0; alive && take_tile(a, worker, workers, i, t); ++i) {
+                const uint32_t buf = i & 1u, br = static_cast<uint32_t>(i) >> 1;
                 if (!mbar_wait_warp(tm_empty(buf), (br & 1u) ^ 1u, abort_flag)) break;
                 tc_fence_after_sync();
                 const uint32_t d_tmem = tmem_base + buf * kBN;
-                for (int st = 0; st < steps; ++st, ++it) {
+                const uint32_t idesc = umma_idesc_bf16(2 * kBM, kBN, false, true) | (t.weight ? 1u << 15 : 0u);
+                // 16 elements of the contraction on: 32 bytes of a K-major row, or two 1024-byte atoms
+                const uint32_t step_a = t.weight ? 2048 >> 4 : 32 >> 4, step_b = 2048 >> 4;
+                for (int st = 0; st < t.kind->steps; ++st, ++it) {
                     const uint32_t s = it % S, r = it / S;
                     if (!mbar_wait_warp(full(s), r & 1u, abort_flag)) { alive = false; break; }
                     tc_fence_after_sync();
                     const uint32_t a_addr = ring + s * kStage;
-                    const uint64_t a_desc = kWeight ? umma_desc_mn_sw128(a_addr, kChunk) : umma_desc_sw128(a_addr);
+                    const uint64_t a_desc = t.weight ? umma_desc_mn_sw128(a_addr, kChunk) : umma_desc_sw128(a_addr);
                     const uint64_t b_desc = umma_desc_mn_sw128(a_addr + 2 * kChunk, kChunk);
-                    // 16 elements of the contraction on: 32 bytes of a K-major row, or two 1024-byte atoms
-                    constexpr uint32_t kStepA = kWeight ? 2048 >> 4 : 32 >> 4, kStepB = 2048 >> 4;
                     if (elect_one()) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            umma_bf16<2>(d_tmem, a_desc + kStepA * j, b_desc + kStepB * j, idesc, (st | j) != 0 ? 1u : 0u);
+                            umma_bf16<2>(d_tmem, a_desc + step_a * j, b_desc + step_b * j, idesc, (st | j) != 0 ? 1u : 0u);
                         umma_commit_2cta(empty(s), 3);
-                        if (st == steps - 1) umma_commit_2cta(tm_full(buf), 3);
+                        if (st == t.kind->steps - 1) umma_commit_2cta(tm_full(buf), 3);
                     }
                     __syncwarp();
                 }
@@ -172,24 +326,29 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
         // ---------------------------------------------------------- epilogue
         const int sp = warp & 3;
         const uint32_t stage0 = st_base + (warp - 2) * 2 * kStoreStage;
-        float alpha = a.num != nullptr ? __ldg(a.num) : 1.0f;
-        if (a.den != nullptr) {
-            const float d = __ldg(a.den);
-            if (d != 0.0f) alpha /= d;
-        }
-        uint32_t local_tile = 0, chunk_no = 0;
-        for (int tile = worker; tile < num_tiles; tile += workers, ++local_tile) {
-            int tm, tn;
-            tile_coord(tile, tm, tn);
-            const uint32_t buf = local_tile & 1u, br = local_tile >> 1;
+        uint32_t chunk_no = 0;
+        Tile t;
+        for (int i = 0; take_tile(a, worker, workers, i, t); ++i) {
+            const uint32_t buf = i & 1u, br = static_cast<uint32_t>(i) >> 1;
+            float alpha = 1.0f;
+            if (t.weight) {
+                if (a.num != nullptr) alpha = __ldg(a.num);
+                if (a.den[t.matrix] != nullptr) {
+                    const float d = __ldg(a.den[t.matrix]);
+                    if (d != 0.0f) alpha /= d;
+                }
+            } else if (a.dx_scale != nullptr) {
+                alpha = __ldg(a.dx_scale);
+            }
+            const CUtensorMap* out = t.weight ? &maps.dw[t.matrix] : &maps.dx;
             if (!mbar_wait_warp(tm_full(buf), br & 1u, abort_flag)) break;
             tc_fence_after_sync();
-            const int row0 = (tm * 2 + static_cast<int>(cta_rank)) * kBM + sp * 32;
+            const int row0 = (t.tm * 2 + static_cast<int>(cta_rank)) * kBM + sp * 32;
             const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(sp * 32) << 16) + buf * kBN;
 #pragma unroll 1
             for (int c = 0; c < kBN; c += 64) {
-                const int col0 = tn * kBN + c;
-                if (row0 >= a.rows || col0 >= a.cols) break;
+                const int col0 = t.tn * kBN + c;
+                if (row0 >= t.kind->rows || col0 >= t.kind->cols) break;
                 uint32_t v[64], h[32];
                 load64(t_addr + c, v);
                 tmem_ld_wait();
@@ -204,7 +363,7 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) {
-                    tma_store_2d(&tm_c, stg, col0, row0);
+                    tma_store_2d(out, stg, col0, row0);
                     tma_store_commit();
                 }
                 ++chunk_no;
@@ -232,124 +391,132 @@ grad_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
     }
 }
 
-// ------------------------------------------------------------------ dg and du
-
-constexpr int kGateThreads = 256;
-
-template <int kAct>
-__device__ __forceinline__ void gate_grad(float dh, float g, float u, float fg, float fu, float& dg, float& du)
+// Pieces of the workspace, each on a 256-byte boundary.
+struct Layout {
+    long long d0 = 0, d1 = 0, w0 = 0, w1 = 0, x = 0, bytes = 0, ld = 0;
+};
+Layout layout(long long m, long long n, long long k, bool gated, bool want_dx, bool want_dw)
 {
-    float act, slope;
-    gate_act_slope<kAct>(g, act, slope);
-    dg = dh * u * slope * fg;
-    du = dh * act * fu;
+    Layout l;
+    l.ld = (n + 7) / 8 * 8;
+    auto piece = [&](long long bytes) { const long long at = l.bytes; l.bytes += (bytes + 255) / 256 * 256; return at; };
+    if (gated || n % 8 != 0) l.d0 = piece(m * l.ld * 2);  // (else dy is read as it is)
+    if (gated) l.d1 = piece(m * l.ld * 2);
+    if (want_dx) { l.w0 = piece(n * k * 2); if (gated) l.w1 = piece(n * k * 2); }
+    if (want_dw) l.x = piece(m * k * 2);
+    return l;
 }
 
-// Eight columns per thread where rows are 16-byte aligned, else one.  Bound by HBM: 10 bytes per element.
-template <int kAct, bool kVec>
-__global__ void __launch_bounds__(kGateThreads)
-gate_backward_kernel(const __nv_bfloat16* __restrict__ dh, const __nv_bfloat16* __restrict__ gate, const __nv_bfloat16* __restrict__ up,
-                     __nv_bfloat16* __restrict__ dg, __nv_bfloat16* __restrict__ du, const float* __restrict__ f_g,
-                     const float* __restrict__ f_u, int m, int n, long long ld)
-{
-    float fg = f_g != nullptr ? __ldg(f_g) : 1.0f, fu = f_u != nullptr ? __ldg(f_u) : 1.0f;
-    if (fg == 0.0f) fg = 1.0f;
-    if (fu == 0.0f) fu = 1.0f;
-    constexpr int kE = kVec ? 8 : 1;
-    const int per_row = n / kE;
-    const long long total = static_cast<long long>(m) * per_row;
-    const long long stride = static_cast<long long>(gridDim.x) * kGateThreads;
-    for (long long i = blockIdx.x * static_cast<long long>(kGateThreads) + threadIdx.x; i < total; i += stride) {
-        const long long row = i / per_row;
-        const int col = static_cast<int>(i - row * per_row) * kE;
-        const size_t src = static_cast<size_t>(row) * n + col, dst = static_cast<size_t>(row) * ld + col;
-        __align__(16) __nv_bfloat16 e_dh[kE], e_g[kE], e_u[kE], o_g[kE], o_u[kE];
-        if constexpr (kVec) {
-            *reinterpret_cast<uint4*>(e_dh) = __ldg(reinterpret_cast<const uint4*>(dh + src));
-            *reinterpret_cast<uint4*>(e_g) = __ldg(reinterpret_cast<const uint4*>(gate + src));
-            *reinterpret_cast<uint4*>(e_u) = __ldg(reinterpret_cast<const uint4*>(up + src));
-        } else {
-            e_dh[0] = dh[src]; e_g[0] = gate[src]; e_u[0] = up[src];
-        }
-#pragma unroll
-        for (int e = 0; e < kE; ++e) {
-            float a, b;
-            gate_grad<kAct>(__bfloat162float(e_dh[e]), __bfloat162float(e_g[e]), __bfloat162float(e_u[e]), fg, fu, a, b);
-            o_g[e] = __float2bfloat16_rn(a);
-            o_u[e] = __float2bfloat16_rn(b);
-        }
-        if constexpr (kVec) {
-            *reinterpret_cast<uint4*>(dg + dst) = *reinterpret_cast<const uint4*>(o_g);
-            *reinterpret_cast<uint4*>(du + dst) = *reinterpret_cast<const uint4*>(o_u);
-        } else {
-            dg[dst] = o_g[0]; du[dst] = o_u[0];
-        }
-    }
-}
+bool unaligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
 
-template <bool kWeight>
-int launch_grad(DeviceCtx* ctx, const GradProduct& p, cudaStream_t stream)
+// The launch may begin while the one before it in the stream ends; the kernels wait before they touch memory.
+void allow_overlap(cudaLaunchConfig_t& cfg, cudaStream_t stream, cudaLaunchAttribute (&attr)[1])
 {
-    GradArgs a = {};
-    a.num = p.num; a.den = p.den;
-    a.rows = kWeight ? p.n : p.m;
-    a.cols = p.k;
-    a.tiles_m = (a.rows + 255) / 256;
-    a.tiles_n = (p.k + kBN - 1) / kBN;
-    a.steps = ((kWeight ? p.m : p.n) + kStepK - 1) / kStepK;
-    a.segments = p.d1 != nullptr ? 2 : 1;
-    a.status = ctx->status_dev;
-    const uint64_t ld_bytes = static_cast<uint64_t>(p.ld) * 2, k_bytes = static_cast<uint64_t>(p.k) * 2;
-    const int b_rows = kWeight ? p.m : p.n;
-    CUtensorMap a0, a1, b0, b1, c;
-    const uint32_t box_a = kWeight ? kStepK : kBM;
-    int rc = encode_tensor_map_2d(ctx, &a0, p.d0, 2, p.n, p.m, ld_bytes, 64, box_a, true);
-    if (rc == INT4L_OK) rc = encode_tensor_map_2d(ctx, &b0, p.b0, 2, p.k, b_rows, k_bytes, 64, kStepK, true);
-    a1 = a0; b1 = b0;
-    if (rc == INT4L_OK && p.d1 != nullptr) {
-        rc = encode_tensor_map_2d(ctx, &a1, p.d1, 2, p.n, p.m, ld_bytes, 64, box_a, true);
-        if (rc == INT4L_OK) rc = encode_tensor_map_2d(ctx, &b1, p.b1, 2, p.k, b_rows, k_bytes, 64, kStepK, true);
-    }
-    if (rc == INT4L_OK) rc = encode_tensor_map_2d(ctx, &c, p.out, 2, p.k, a.rows, k_bytes, 64, 32, true);
-    if (rc != INT4L_OK) return rc;
-    const long long tiles = static_cast<long long>(a.tiles_m) * a.tiles_n;
-    const int pairs = tiles < ctx->max_pairs ? static_cast<int>(tiles) : ctx->max_pairs;
-    grad_gemm_kernel<kWeight><<<pairs * 2, kThreads, kSmemBytes, stream>>>(a0, a1, b0, b1, c, a);
+    cfg.stream = stream;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
     count_launch();
-    return cudaGetLastError() == cudaSuccess ? INT4L_OK : INT4L_ERR_CUDA;
 }
 
 }  // namespace
 
-int setup_grad(DeviceCtx*)
+long long fp4_backward_workspace(long long m, long long n, long long k, bool gated, bool want_dx, bool want_dw)
 {
-    const bool ok = cudaFuncSetAttribute(grad_gemm_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) == cudaSuccess &&
-                    cudaFuncSetAttribute(grad_gemm_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) == cudaSuccess;
-    return ok ? INT4L_OK : INT4L_ERR_CUDA;
+    return layout(m, n, k, gated, want_dx, want_dw).bytes;
 }
 
-int launch_grad_product(DeviceCtx* ctx, const GradProduct& p, cudaStream_t stream)
+int setup_fp4_backward(DeviceCtx*)
 {
-    return p.weight ? launch_grad<true>(ctx, p, stream) : launch_grad<false>(ctx, p, stream);
+    return cudaFuncSetAttribute(grad_gemm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) == cudaSuccess ? INT4L_OK : INT4L_ERR_CUDA;
 }
 
-int launch_gate_backward(DeviceCtx* ctx, const void* dh, const void* gate, const void* up, void* dg, void* du, int act,
-                         const float* f_g, const float* f_u, int m, int n, long long ld, cudaStream_t stream)
+int launch_fp4_backward(DeviceCtx* ctx, const Fp4Backward& b, cudaStream_t stream)
 {
     using B = __nv_bfloat16;
-    const bool vec = n % 8 == 0 && ((reinterpret_cast<uintptr_t>(dh) | reinterpret_cast<uintptr_t>(gate) | reinterpret_cast<uintptr_t>(up)) & 15u) == 0;
-    const long long units = static_cast<long long>(m) * (vec ? n / 8 : n);
-    const long long blocks = (units + kGateThreads - 1) / kGateThreads, cap = static_cast<long long>(ctx->sm_count) * 32;
-    const int grid = static_cast<int>(blocks < cap ? blocks : cap);
-    auto go = [&](auto kernel) {
-        kernel<<<grid, kGateThreads, 0, stream>>>(static_cast<const B*>(dh), static_cast<const B*>(gate), static_cast<const B*>(up),
-                                                  static_cast<B*>(dg), static_cast<B*>(du), f_g, f_u, m, n, ld);
+    const Fp4Problem& p = b.forward;
+    const Layout l = layout(p.m, p.n, p.k, p.gated, b.dx != nullptr, b.dw != nullptr);
+    uint8_t* ws = b.workspace;
+    const bool direct = !p.gated && p.n % 8 == 0;  // dy as it is
+    const void* d[2] = {direct ? b.dy : ws + l.d0, ws + l.d1};
+
+    // ------------------------------------------------------------ preparation
+    PrepArgs pa = {};
+    long long blocks = 0;
+    if (!direct) {
+        pa.gate = GateJob{static_cast<const B*>(b.dy), static_cast<const B*>(b.gate), static_cast<const B*>(b.up),
+                          reinterpret_cast<B*>(ws + l.d0), reinterpret_cast<B*>(ws + l.d1), p.w.tensor_scale, p.w_up.tensor_scale,
+                          p.m, p.n, p.act, p.n % 8 == 0 && !unaligned16(b.dy) && !unaligned16(b.gate) && !unaligned16(b.up), l.ld};
+        const long long units = static_cast<long long>(p.m) * ((p.n + 255) / 256);
+        if (units > 0xFFFFFFFFll - 8) return INT4L_ERR_TOO_LARGE;
+        blocks = (units + kUnitThreads / 32 - 1) / (kUnitThreads / 32);
+    }
+    int jobs = 0;
+    auto expand = [&](const Fp4& q, long long at) {
+        pa.first[jobs] = static_cast<uint32_t>(blocks);
+        pa.expand[jobs++] = ExpandJob{q.codes, q.scales, q.tensor_scale, reinterpret_cast<B*>(ws + at), q.rows, q.k};
+        blocks += fp4_expand_blocks(q.rows, q.k);
     };
-    if (act == kActSilu) vec ? go(gate_backward_kernel<kActSilu, true>) : go(gate_backward_kernel<kActSilu, false>);
-    else if (act == kActGelu) vec ? go(gate_backward_kernel<kActGelu, true>) : go(gate_backward_kernel<kActGelu, false>);
-    else vec ? go(gate_backward_kernel<kActGeluTanh, true>) : go(gate_backward_kernel<kActGeluTanh, false>);
-    count_launch();
-    return cudaGetLastError() == cudaSuccess ? INT4L_OK : INT4L_ERR_CUDA;
+    if (b.dx) {
+        expand(p.w, l.w0);
+        if (p.gated) expand(p.w_up, l.w1);
+    }
+    if (b.dw) expand(p.x, l.x);
+    if (blocks > 0x7FFFFFFF) return INT4L_ERR_TOO_LARGE;
+    for (int i = jobs; i < 4; ++i) pa.first[i] = static_cast<uint32_t>(blocks);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    cfg.gridDim = dim3(static_cast<unsigned>(blocks), 1, 1);
+    cfg.blockDim = dim3(kUnitThreads, 1, 1);
+    allow_overlap(cfg, stream, attr);
+    if (cudaLaunchKernelEx(&cfg, p.x.block16 ? backward_prepare_kernel<true> : backward_prepare_kernel<false>, pa) != cudaSuccess) {
+        cudaGetLastError();
+        return INT4L_ERR_CUDA;
+    }
+
+    // --------------------------------------------------------------- products
+    GradArgs a = {};
+    Maps maps;
+    const int matrices = p.gated ? 2 : 1;
+    const int steps_n = (p.n + kStepK - 1) / kStepK, steps_m = (p.m + kStepK - 1) / kStepK;
+    const Kind dx = {0, 1, p.m, p.k, (p.m + 255) / 256, (p.k + kBN - 1) / kBN, matrices * steps_n};
+    const Kind dw = {1, matrices, p.n, p.k, (p.n + 255) / 256, (p.k + kBN - 1) / kBN, steps_m};
+    const long long tiles_dx = b.dx ? static_cast<long long>(dx.tiles_m) * dx.tiles_n : 0;
+    const long long tiles_dw = b.dw ? static_cast<long long>(matrices) * dw.tiles_m * dw.tiles_n : 0;
+    if (tiles_dx + tiles_dw > (1 << 30)) return INT4L_ERR_TOO_LARGE;
+    const bool dx_first = tiles_dw == 0 || (tiles_dx > 0 && dx.steps >= dw.steps);
+    a.kind[0] = dx_first ? dx : dw;
+    a.kind[1] = dx_first ? dw : dx;
+    a.tiles[0] = static_cast<int>(dx_first ? tiles_dx : tiles_dw);
+    a.tiles[1] = static_cast<int>(dx_first ? tiles_dw : tiles_dx);
+    a.segment = steps_n;
+    const int workers = tiles_dx + tiles_dw < ctx->max_pairs ? static_cast<int>(tiles_dx + tiles_dw) : ctx->max_pairs;
+    a.extra = a.tiles[0] % workers == 0 ? 0 : (a.kind[0].steps + a.kind[1].steps / 2) / a.kind[1].steps;
+    a.num = p.x.tensor_scale;
+    if (p.gated) { a.den[0] = p.w.tensor_scale; a.den[1] = p.w_up.tensor_scale; }
+    else a.dx_scale = p.w.tensor_scale;
+    a.status = ctx->status_dev;
+    const uint64_t d_pitch = direct ? static_cast<uint64_t>(p.n) * 2 : static_cast<uint64_t>(l.ld) * 2, k_pitch = static_cast<uint64_t>(p.k) * 2;
+    int rc = INT4L_OK;
+    auto map = [&](CUtensorMap* out, const void* at, int cols, int rows, uint64_t pitch, int box_rows) {
+        if (rc == INT4L_OK) rc = encode_tensor_map_2d(ctx, out, at, 2, cols, rows, pitch, 64, box_rows, true);
+    };
+    for (int i = 0; i < matrices; ++i) {
+        map(&maps.d[i], d[i], p.n, p.m, d_pitch, 64);
+        if (b.dx) map(&maps.w[i], ws + (i ? l.w1 : l.w0), p.k, p.n, k_pitch, 64);
+        if (b.dw) map(&maps.dw[i], i ? b.dw_up : b.dw, p.k, p.n, k_pitch, 32);
+    }
+    if (b.dw) map(&maps.x, ws + l.x, p.k, p.m, k_pitch, 64);
+    if (b.dx) map(&maps.dx, b.dx, p.k, p.m, k_pitch, 32);
+    if (rc != INT4L_OK) return rc;
+    cudaLaunchConfig_t cfg2 = {};
+    cfg2.gridDim = dim3(workers * 2, 1, 1);
+    cfg2.blockDim = dim3(kThreads, 1, 1);
+    cfg2.dynamicSmemBytes = kSmemBytes;
+    allow_overlap(cfg2, stream, attr);
+    if (cudaLaunchKernelEx(&cfg2, grad_gemm_kernel, maps, a) != cudaSuccess) { cudaGetLastError(); return INT4L_ERR_CUDA; }
+    return INT4L_OK;
 }
 
 }  // namespace i4l
