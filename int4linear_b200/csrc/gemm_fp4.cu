@@ -132,6 +132,7 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
     const int worker = static_cast<int>(cluster_id_x());
     const int workers = static_cast<int>(cluster_count_x());
 
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (tid == 0) {
         for (int i = 0; i < S; ++i) { mbar_init(full(i), 1); mbar_init(empty(i), 1); }
         mbar_init(acc_full, 1);
@@ -151,6 +152,8 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
     cluster_sync_all();
     tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot;
+    // Everything above may run while the launch before this one in the stream ends.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
 
     const int num_tiles = a.tiles_m * a.tiles_n;
     const int steps = (a.k + kStepK - 1) / kStepK;
@@ -351,10 +354,21 @@ int launch_cfg(DeviceCtx* ctx, const Fp4Problem& p, cudaStream_t stream)
     const long long tiles = static_cast<long long>(a.tiles_m) * a.tiles_n;
     if (tiles > (1 << 30)) return INT4L_ERR_TOO_LARGE;
     const int pairs = tiles < ctx->max_pairs ? static_cast<int>(tiles) : ctx->max_pairs;
-    gemm_fp4_kernel<kBlock16, kGated, kHalf><<<pairs * 2, kThreads, Geo<kBlock16>::kSmemBytes, stream>>>(
-        tm_x, tm_w, tm_w_up, tm_sx, tm_sw, tm_sw_up, tm_y, tm_g, tm_u, a);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(pairs * 2, 1, 1);
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = Geo<kBlock16>::kSmemBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_fp4_kernel<kBlock16, kGated, kHalf>, tm_x, tm_w, tm_w_up, tm_sx, tm_sw, tm_sw_up,
+                                             tm_y, tm_g, tm_u, a);
     count_launch();
-    return cudaGetLastError() == cudaSuccess ? INT4L_OK : INT4L_ERR_CUDA;
+    if (e != cudaSuccess) { cudaGetLastError(); return INT4L_ERR_CUDA; }
+    return INT4L_OK;
 }
 
 template <bool kBlock16, bool kGated>
