@@ -46,8 +46,7 @@ bool bad_act(int act) { return act != INT4L_ACT_SILU && act != INT4L_ACT_GELU &&
 
 int launch_product(DeviceCtx* ctx, const Fp4Problem& p, cudaStream_t stream)
 {
-    const bool few = fp4_fewrows_supports(p) && (p.m <= 64);
-    return few ? launch_fp4_fewrows(ctx, p, stream) : launch_fp4_gemm(ctx, p, stream);
+    return fp4_fewrows_preferred(ctx, p) ? launch_fp4_fewrows(ctx, p, stream) : launch_fp4_gemm(ctx, p, stream);
 }
 
 // The common part of both backward passes.

@@ -73,7 +73,7 @@ int setup_fp4_gemm(DeviceCtx* ctx);
 int launch_fp4_gemm(DeviceCtx* ctx, const Fp4Problem& p, cudaStream_t stream);
 // Few rows of x (gemm_fp4_fewrows.cu).
 int setup_fp4_fewrows(DeviceCtx* ctx);
-bool fp4_fewrows_supports(const Fp4Problem& p);
+bool fp4_fewrows_preferred(const DeviceCtx* ctx, const Fp4Problem& p);
 int launch_fp4_fewrows(DeviceCtx* ctx, const Fp4Problem& p, cudaStream_t stream);
 
 }  // namespace i4l

@@ -1,4 +1,4 @@
-// The products of gemm_fp4.cu for few rows of x (decode batches, up to 128 rows): a stream of the weights.
+// The products of gemm_fp4.cu for few rows of x (decode batches): a stream of the weights.
 //
 // Every byte of w is used once, so the time is that of bringing w in, and nearly all SMs have to take part from the
 // start.  The operands are swapped: the UMMA's 128-row side holds rows of w, its narrow side the rows of x (padded to
@@ -54,6 +54,7 @@ struct Args {
     int n_pad;     // rows of x in the UMMA, a multiple of 16
     int stages, stage_bytes, cols;
     int split;     // CTAs per cluster
+    int tiles;     // of 128 rows of w
     int act, fp16;
     int* status;
 };
@@ -105,7 +106,10 @@ gemm_fp4_fewrows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int split = a.split;
     const int rank = static_cast<int>(blockIdx.x) % split;
-    const int tile = static_cast<int>(blockIdx.x) / split;
+    const int item = static_cast<int>(blockIdx.x) / split;
+    const int tile = item % a.tiles, group = item / a.tiles;  // 128 rows of w, 128 rows of x
+    const int m = min(128, a.m - group * 128);                // (of x, here)
+    const size_t out0 = static_cast<size_t>(group) * 128 * a.n;
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (tid == 0) {
@@ -149,8 +153,8 @@ gemm_fp4_fewrows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
                 if (kGated) tma_load_2d(dst + G::kCodesW, &tm_w_up, full(s), kb * kStepBytes, tile * kRows);
                 tma_load_2d(dst + G::kOffScales, &tm_sw, full(s), sc, tile);
                 if (kGated) tma_load_2d(dst + G::kOffScales + G::kScaleBytes, &tm_sw_up, full(s), sc, tile);
-                tma_load_2d(dst + G::kOffScales + G::kW * G::kScaleBytes, &tm_sx, full(s), sc, 0);
-                tma_load_2d(dst + G::kOffX, &tm_x, full(s), kb * kStepBytes, 0);
+                tma_load_2d(dst + G::kOffScales + G::kW * G::kScaleBytes, &tm_sx, full(s), sc, group);
+                tma_load_2d(dst + G::kOffX, &tm_x, full(s), kb * kStepBytes, group * 128);
             }
             __syncwarp();
             if (++s == a.stages) { s = 0; phase ^= 1u; }
@@ -199,7 +203,7 @@ gemm_fp4_fewrows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
     auto bits = [&](float v) { return scaled_to_bits(v, a.fp16); };
     // One value of y, from its sum (or its two) and, for a product, its column's bias.
     auto put = [&](int i, int col, float acc, float acc_up, float bias) {
-        const size_t at = static_cast<size_t>(i) * a.n + col;
+        const size_t at = out0 + static_cast<size_t>(i) * a.n + col;
         if constexpr (kGated) {
             const float g = acc * alpha, u = acc_up * alpha_up;
             a.y[at] = bits(act_of(g, a.act) * u);
@@ -215,7 +219,7 @@ gemm_fp4_fewrows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
         const int col = tile * kRows + tid;
         const float bias = split == 1 ? bias_of(col) : 0.0f;
 #pragma unroll 1
-        for (int c = 0; c < a.n_pad && c < a.m; c += 16) {
+        for (int c = 0; c < m; c += 16) {
             uint32_t v[G::kW][16];
 #pragma unroll
             for (int i = 0; i < G::kW; ++i) tmem_ld_16(lanes + i * a.n_pad + c, v[i]);
@@ -224,7 +228,7 @@ gemm_fp4_fewrows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
                 if (col < a.n) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
-                        if (c + e < a.m) put(c + e, col, __uint_as_float(v[0][e]), __uint_as_float(v[G::kW - 1][e]), bias);
+                        if (c + e < m) put(c + e, col, __uint_as_float(v[0][e]), __uint_as_float(v[G::kW - 1][e]), bias);
                 }
             } else {
 #pragma unroll
@@ -246,7 +250,7 @@ gemm_fp4_fewrows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
         for (int e = 0; e < 4; ++e) bias[e] = bias_of(col + e);
         if (ok) {
 #pragma unroll 2
-            for (int i = warp * split + rank; i < a.m; i += 4 * split) {
+            for (int i = warp * split + rank; i < m; i += 4 * split) {
                 float4 sum[G::kW];
 #pragma unroll
                 for (int w = 0; w < G::kW; ++w) {
@@ -276,7 +280,7 @@ gemm_fp4_fewrows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
                         }
                     }
                     auto store4 = [&](unsigned short* dst, const unsigned short (&t)[4]) {
-                        *reinterpret_cast<uint2*>(dst + static_cast<size_t>(i) * a.n + col) =
+                        *reinterpret_cast<uint2*>(dst + out0 + static_cast<size_t>(i) * a.n + col) =
                             make_uint2(t[0] | (static_cast<uint32_t>(t[1]) << 16), t[2] | (static_cast<uint32_t>(t[3]) << 16));
                     };
                     store4(a.y, h);
@@ -324,13 +328,18 @@ int launch_cfg(DeviceCtx* ctx, const Fp4Problem& p, cudaStream_t stream)
     a.keep_gate = static_cast<unsigned short*>(p.keep_gate);
     a.keep_up = static_cast<unsigned short*>(p.keep_up);
     a.m = p.m; a.n = p.n; a.k = p.k;
-    a.n_pad = (p.m + 15) / 16 * 16;
+    a.n_pad = p.m >= 128 ? 128 : (p.m + 15) / 16 * 16;
+    const int groups = (p.m + 127) / 128;
     a.act = p.act;
     a.fp16 = p.fp16;
     a.status = ctx->status_dev;
     const int tiles = (p.n + kRows - 1) / kRows;
     const int steps = (p.k + kStepK - 1) / kStepK;
-    int split = 2 * ctx->sm_count / tiles;
+    a.tiles = tiles;
+    // About two CTAs per SM.  More rows of x make the reduction the larger part: a CTA then takes at least 4 steps
+    // (64 x 4096 x 4096 mxfp4: 7.9 us with 4 CTAs to a tile, 8.7 with 8; 16 rows: 6.3 and 6.2).
+    int split = 2 * ctx->sm_count / (tiles * groups);
+    if (a.n_pad > 32 && split > steps / 4) split = steps / 4;
     split = split < 1 ? 1 : (split > 8 ? 8 : split);
     if (split > steps) split = steps;
     a.split = split;
@@ -371,7 +380,7 @@ int launch_cfg(DeviceCtx* ctx, const Fp4Problem& p, cudaStream_t stream)
     if (rc != INT4L_OK) return rc;
 
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(tiles * split, 1, 1);
+    cfg.gridDim = dim3(tiles * split * groups, 1, 1);
     cfg.blockDim = dim3(kThreads, 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
@@ -403,7 +412,16 @@ int setup_fp4_fewrows(DeviceCtx*)
     return set_attr<false, false>() && set_attr<false, true>() && set_attr<true, false>() && set_attr<true, true>() ? INT4L_OK : INT4L_ERR_CUDA;
 }
 
-bool fp4_fewrows_supports(const Fp4Problem& p) { return p.m <= 128; }
+// Up to 64 rows this kernel is the faster one everywhere (64 x 14336 x 4096: 11.5 us against 11.9; 1 x 4096 x 4096: 6.1
+// against 8.2), from there on only where the tiles of gemm_fp4.cu leave most SMs idle for a long k: 128 x 1024 x 8192
+// 8.9 us against 13.9, 256 x 1024 x 8192 10.1 against 14.8, but 128 x 1024 x 1024 7.1 against 5.2 and 256 x 4096 x 4096
+// 10.8 against 9.9.  A gated tile has twice the partial sums to exchange and does not profit.
+bool fp4_fewrows_preferred(const DeviceCtx* ctx, const Fp4Problem& p)
+{
+    if (p.m <= 64) return true;
+    const int tiles = (p.n + kRows - 1) / kRows * ((p.m + 127) / 128);
+    return !p.gated && p.m <= 256 && p.k > 6144 && tiles <= ctx->sm_count / 4;
+}
 
 int launch_fp4_fewrows(DeviceCtx* ctx, const Fp4Problem& p, cudaStream_t stream)
 {

@@ -104,7 +104,7 @@ class Fp4Matrix:
         """An uninitialised matrix, its arguments already checked."""
         import torch
         q = object.__new__(cls)
-        q.__dict__.update(codes=torch.empty((rows, k // 2), dtype=torch.uint8, device=device),
+        q.__dict__.update(codes=torch.empty(rows, k // 2, dtype=torch.uint8, device=device),
                           scales=torch.empty(_scale_bytes(rows, k, fmt), dtype=torch.uint8, device=device),
                           rows=rows, k=k, format=fmt, tensor_scale=tensor_scale)
         q._wrap()
@@ -236,7 +236,7 @@ def dequantize_fp4(q: Fp4Matrix, dtype=None, out=None, stream=None):
         _check_out(out, q.shape, dtype, q.device)
 
     def body(handle):
-        y = out if out is not None else torch.empty((q.rows, q.k), dtype=dtype, device=q.device)
+        y = out if out is not None else torch.empty(q.rows, q.k, dtype=dtype, device=q.device)
         if q.rows:
             _check(_lib.load().int4_linear_fp4_dequantize_async(q._p, y.data_ptr(), t, handle), "int4_linear_fp4_dequantize_async")
         return y
@@ -282,7 +282,7 @@ def linear_fp4(x: Fp4Matrix, w: Fp4Matrix, bias=None, out=None, dtype=None, stre
         _check_out(out, (m, n), dtype, x.device)
 
     def body(handle):
-        y = out if out is not None else torch.empty((m, n), dtype=dtype, device=x.device)
+        y = out if out is not None else torch.empty(m, n, dtype=dtype, device=x.device)
         if m and n:
             _check(_lib.load().int4_linear_fp4_launch_async(x._p, w._p, bias.data_ptr() if bias is not None else None, y.data_ptr(),
                                                             t, handle), "int4_linear_fp4_launch_async")
@@ -305,7 +305,7 @@ def gated_linear_fp4(x: Fp4Matrix, w_gate: Fp4Matrix, w_up: Fp4Matrix, activatio
         _check_out(out, (m, n), dtype, x.device)
 
     def body(handle):
-        h = out if out is not None else torch.empty((m, n), dtype=dtype, device=x.device)
+        h = out if out is not None else torch.empty(m, n, dtype=dtype, device=x.device)
         gate, up = (torch.empty_like(h), torch.empty_like(h)) if save else (None, None)
         if m and n:
             _check(_lib.load().int4_linear_fp4_gated_launch_async(
@@ -339,8 +339,8 @@ def linear_fp4_backward(grad_y, x: Fp4Matrix, w: Fp4Matrix, need=(True, True), s
     def body(handle):
         empty = m == 0 or n == 0  # an empty sum is 0
         new = torch.zeros if empty else torch.empty
-        dx = new((m, x.k), dtype=torch.bfloat16, device=x.device) if want_x else None
-        dw = new((n, x.k), dtype=torch.bfloat16, device=x.device) if want_w else None
+        dx = new(m, x.k, dtype=torch.bfloat16, device=x.device) if want_x else None
+        dw = new(n, x.k, dtype=torch.bfloat16, device=x.device) if want_w else None
         if not empty and (want_x or want_w):
             dy = grad_y.contiguous()
             if dy.data_ptr() % 16:
@@ -371,9 +371,9 @@ def gated_linear_fp4_backward(grad_h, gate, up, x: Fp4Matrix, w_gate: Fp4Matrix,
     def body(handle):
         empty = m == 0 or n == 0
         new = torch.zeros if empty else torch.empty
-        dx = new((m, x.k), dtype=torch.bfloat16, device=x.device) if want_x else None
-        dwg = new((n, x.k), dtype=torch.bfloat16, device=x.device) if want_w else None
-        dwu = new((n, x.k), dtype=torch.bfloat16, device=x.device) if want_w else None
+        dx = new(m, x.k, dtype=torch.bfloat16, device=x.device) if want_x else None
+        dwg = new(n, x.k, dtype=torch.bfloat16, device=x.device) if want_w else None
+        dwu = new(n, x.k, dtype=torch.bfloat16, device=x.device) if want_w else None
         if not empty and (want_x or want_w):
             dh, g, u = grad_h.contiguous(), gate.contiguous(), up.contiguous()
             ws = _workspace(m, n, x.k, True, want_x, want_w, x.device)

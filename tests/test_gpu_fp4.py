@@ -167,7 +167,7 @@ def test_scale_order_round_trip(cuda):
 
 SHAPES = [(1, 1, 32), (1, 128, 256), (2, 40, 64), (16, 14336 // 16, 4096), (5, 250, 992), (31, 64, 96), (33, 129, 160),
           (64, 1000, 512), (100, 77, 288), (128, 256, 256), (129, 257, 1056), (200, 512, 2080), (257, 385, 544),
-          (300, 1024, 8192), (513, 520, 32)]
+          (300, 1024, 8192), (513, 520, 32), (65, 200, 6400), (129, 1000, 8192), (256, 130, 14336)]
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
