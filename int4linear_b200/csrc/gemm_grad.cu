@@ -23,11 +23,12 @@
 //
 // dx and dw tiles have contractions of different length (n or 2 n, and m), and with separate launches each product
 // leaves a partly filled last wave.  Together they are dealt out in advance: the longer kind round-robin, the shorter
-// kind first to the workers that got one fewer, then round-robin (4096 x 14336 x 4096: 24 + 26 -> 49 of 46.5 waves of
-// the weight gradients' tile time).
+// kind first to the workers that got one fewer, then round-robin (grad_schedule.cuh; gated 4096 x 14336 x 4096 on 74
+// pairs, in tile times of the weight gradients: 28 + 13 + 13 apart, 49 together, 48.4 the mean).
 #include "epilogue.cuh"
 #include "fp4_expand.cuh"
 #include "gate.cuh"
+#include "grad_schedule.cuh"
 #include "ptx.cuh"
 
 namespace i4l {
@@ -162,9 +163,8 @@ struct Kind {
 };
 struct GradArgs {
     Kind kind[2];           // the one with the longer contraction first; kind[1] may have no tiles
-    int tiles[2];
+    Deal deal;
     int segment;            // dx: steps of the first of its two contractions
-    int extra;              // tiles of kind 1 that a worker with one fewer of kind 0 takes first
     const float* num; const float* den[2];  // dw[i] *= num / den[i]
     const float* dx_scale;                  // dx *= this
     int* status;
@@ -173,26 +173,6 @@ struct Maps {
     CUtensorMap d[2], w[2], x, dx, dw[2];
 };
 
-// The i-th tile of a worker: its kind and index; false when there is none.
-__device__ __forceinline__ bool tile_of(const GradArgs& a, int worker, int workers, int i, int& kind, int& tile)
-{
-    const int mine = worker < a.tiles[0] ? (a.tiles[0] - worker + workers - 1) / workers : 0;
-    if (i < mine) { kind = 0; tile = worker + i * workers; return true; }
-    kind = 1;
-    i -= mine;
-    const int full = a.tiles[0] % workers;  // workers [full, workers) have one tile of kind 0 fewer
-    const int few = workers - full;
-    const int dealt = min(static_cast<long long>(few) * a.extra, static_cast<long long>(a.tiles[1]));
-    if (worker >= full) {
-        const int at = worker - full, own = at < dealt ? (dealt - at + few - 1) / few : 0;
-        if (i < own) { tile = at + i * few; return true; }
-        i -= own;
-    }
-    const long long t = dealt + worker + static_cast<long long>(i) * workers;
-    tile = static_cast<int>(t);
-    return t < a.tiles[1];
-}
-
 struct Tile {
     const Kind* kind;
     int weight, matrix, tm, tn;
@@ -200,7 +180,7 @@ struct Tile {
 __device__ __forceinline__ bool take_tile(const GradArgs& a, int worker, int workers, int i, Tile& t)
 {
     int kind, tile;
-    if (!tile_of(a, worker, workers, i, kind, tile)) return false;
+    if (!a.deal.tile_of(worker, workers, i, kind, tile)) return false;
     const Kind& k = a.kind[kind];
     t.kind = &k;
     t.weight = k.weight;
@@ -488,11 +468,10 @@ int launch_fp4_backward(DeviceCtx* ctx, const Fp4Backward& b, cudaStream_t strea
     const bool dx_first = tiles_dw == 0 || (tiles_dx > 0 && dx.steps >= dw.steps);
     a.kind[0] = dx_first ? dx : dw;
     a.kind[1] = dx_first ? dw : dx;
-    a.tiles[0] = static_cast<int>(dx_first ? tiles_dx : tiles_dw);
-    a.tiles[1] = static_cast<int>(dx_first ? tiles_dw : tiles_dx);
     a.segment = steps_n;
     const int workers = tiles_dx + tiles_dw < ctx->max_pairs ? static_cast<int>(tiles_dx + tiles_dw) : ctx->max_pairs;
-    a.extra = a.tiles[0] % workers == 0 ? 0 : (a.kind[0].steps + a.kind[1].steps / 2) / a.kind[1].steps;
+    a.deal = deal_tiles(static_cast<int>(dx_first ? tiles_dx : tiles_dw), static_cast<int>(dx_first ? tiles_dw : tiles_dx), a.kind[0].steps,
+                        a.kind[1].steps, workers);
     a.num = p.x.tensor_scale;
     if (p.gated) { a.den[0] = p.w.tensor_scale; a.den[1] = p.w_up.tensor_scale; }
     else a.dx_scale = p.w.tensor_scale;
