@@ -6,10 +6,12 @@
 //
 // with respect to the values the operands stand for.  The contraction runs over n or m, across the blocks that
 // share a scale, so the block-scaled instruction does not apply: the operands are expanded to bf16 first.  That
-// loses nothing (a code times its e8m0 or e4m3 scale has at most 6 significant bits); only the incoming gradient
-// is rounded, dg and du to bf16, as the gradients of a bf16 network are.
+// loses nothing (a code times its e8m0 or e4m3 scale has at most 6 significant bits).  Only dg and du are rounded, to
+// bf16 as the gradients of a bf16 network are: with the rounding of the result that is 1.4 times the error of one
+// rounding (2.4e-3 in the mean square against 1.7e-3).  Where it costs next to nothing (plan() says when) they are
+// carried as the sum of two bf16 values instead, 16 bits, as contractions of twice the length.
 //
-// Two launches.  The first prepares: dg and du (or dy with a row pitch that TMA takes), and the expansions.  The second
+// Two launches, or three.  The first prepares: dg and du (or dy with a row pitch that TMA takes), and the expansions.  The second
 // is all products in one persistent kernel, a CTA pair per 256 x 256 tile (tcgen05.mma kind::f16, cta_group::2), two
 // accumulators in tensor memory so that the epilogue overlaps the next tile:
 //     warp 0      TMA, steps of 64 along the contraction, into 128-byte-swizzled slots
@@ -17,6 +19,10 @@
 //     warps 2-5   epilogue: scale, round to bf16, staged TMA stores
 // No operand is ever transposed: where the contraction runs down the rows of a matrix (w and x always, dy for
 // dw), its tile is read as it lies and the UMMA takes it MN-major.
+//
+// Where the tiles are too few to occupy the GPU for their length (few tokens, so that dx is a handful of tiles of a
+// contraction over all columns), contractions are cut into parts; the parts' fp32 sums go to the workspace, and a third
+// launch adds them in order, so that the result does not depend on timing.
 //
 // The tensor scales are kept out of the expanded matrices.  dx = dg wg + du wu is one contraction over both, so dg and
 // du are multiplied by their weight's tensor scale before they are rounded, and the weight gradients take it out again.
@@ -41,6 +47,7 @@ namespace {
 struct GateJob {
     const __nv_bfloat16* dh; const __nv_bfloat16* gate; const __nv_bfloat16* up;
     __nv_bfloat16* dg; __nv_bfloat16* du;
+    __nv_bfloat16* dg_lo; __nv_bfloat16* du_lo;  // what the rounding left, rounded again; or null
     const float* f_g; const float* f_u;
     int m, n, act, vec;
     long long ld;
@@ -66,6 +73,13 @@ __device__ __forceinline__ void gate_grad(float dh, float g, float u, float fg, 
     du = dh * act * fu;
 }
 
+// What rounding v to `first` left (nothing to add to an infinity).
+__device__ __forceinline__ __nv_bfloat16 second_term(float v, __nv_bfloat16 first)
+{
+    const float f = __bfloat162float(first);
+    return __float2bfloat16_rn(isinf(f) ? 0.0f : v - f);
+}
+
 // A warp's unit: 256 columns of one row, eight per lane (consecutive where 16-byte accesses are possible, else 32
 // apart).  Bound by HBM: 10 bytes per element.
 template <int kAct>
@@ -79,31 +93,42 @@ __device__ __forceinline__ void gate_block(const GateJob& j, uint32_t block)
     float fg = j.f_g != nullptr ? __ldg(j.f_g) : 1.0f, fu = j.f_u != nullptr ? __ldg(j.f_u) : 1.0f;
     if (fg == 0.0f) fg = 1.0f;
     if (fu == 0.0f) fu = 1.0f;
-    __align__(16) __nv_bfloat16 h[8] = {}, g[8] = {}, up[8] = {}, og[8], ou[8];
+    __align__(16) __nv_bfloat16 h[8] = {}, g[8] = {}, up[8] = {}, og[8], ou[8], lg[8], lu[8];
     auto one = [&](int e) {
         float a, b;
         gate_grad<kAct>(__bfloat162float(h[e]), __bfloat162float(g[e]), __bfloat162float(up[e]), fg, fu, a, b);
         og[e] = __float2bfloat16_rn(a);
         ou[e] = __float2bfloat16_rn(b);
+        lg[e] = second_term(a, og[e]);
+        lu[e] = second_term(b, ou[e]);
     };
     if (j.vec) {
         const int col = col0 + lane * 8;
         if (col >= j.n) return;
-        *reinterpret_cast<uint4*>(h) = __ldg(reinterpret_cast<const uint4*>(j.dh + src + col));
-        *reinterpret_cast<uint4*>(g) = __ldg(reinterpret_cast<const uint4*>(j.gate + src + col));
-        *reinterpret_cast<uint4*>(up) = __ldg(reinterpret_cast<const uint4*>(j.up + src + col));
+        auto load = [&](const __nv_bfloat16* p) { return __ldg(reinterpret_cast<const uint4*>(p + src + col)); };
+        auto store = [&](__nv_bfloat16* p, const __nv_bfloat16 (&v)[8]) { *reinterpret_cast<uint4*>(p + dst + col) = *reinterpret_cast<const uint4*>(v); };
+        *reinterpret_cast<uint4*>(h) = load(j.dh);
+        *reinterpret_cast<uint4*>(g) = load(j.gate);
+        *reinterpret_cast<uint4*>(up) = load(j.up);
 #pragma unroll
         for (int e = 0; e < 8; ++e) one(e);
-        *reinterpret_cast<uint4*>(j.dg + dst + col) = *reinterpret_cast<const uint4*>(og);
-        *reinterpret_cast<uint4*>(j.du + dst + col) = *reinterpret_cast<const uint4*>(ou);
+        store(j.dg, og);
+        store(j.du, ou);
+        if (j.dg_lo != nullptr) { store(j.dg_lo, lg); store(j.du_lo, lu); }
     } else {
         const int col = col0 + lane;
 #pragma unroll
         for (int e = 0; e < 8; ++e)
             if (col + 32 * e < j.n) { h[e] = j.dh[src + col + 32 * e]; g[e] = j.gate[src + col + 32 * e]; up[e] = j.up[src + col + 32 * e]; }
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (col + 32 * e < j.n) { one(e); j.dg[dst + col + 32 * e] = og[e]; j.du[dst + col + 32 * e] = ou[e]; }
+        for (int e = 0; e < 8; ++e) {
+            if (col + 32 * e >= j.n) break;
+            one(e);
+            const size_t at = dst + col + 32 * e;
+            j.dg[at] = og[e];
+            j.du[at] = ou[e];
+            if (j.dg_lo != nullptr) { j.dg_lo[at] = lg[e]; j.du_lo[at] = lu[e]; }
+        }
     }
 }
 
@@ -154,28 +179,41 @@ constexpr int kNumBarriers = 2 * kStages + 4;
 constexpr int kSmemBytes = 1024 + kStages * kStage + 4 * 2 * kStoreStage + kNumBarriers * 8 + 16;
 static_assert(kSmemBytes <= 232448, "shared memory budget");
 
-// One kind of tile: dx (its A operand is K-major), or a weight gradient (`matrices` of them, A MN-major).
+// One kind of tile: dx (its A operand is K-major), or a weight gradient (`matrices` of them, A MN-major).  A contraction
+// is `segments` runs of `seg_steps` steps, each over operands of its own, cut into `parts`.
 struct Kind {
     int weight, matrices;
     int rows, cols;         // of one result
     int tiles_m, tiles_n;   // of one result
-    int steps;              // of a whole contraction
+    int segments, seg_steps, parts;
 };
 struct GradArgs {
     Kind kind[2];           // the one with the longer contraction first; kind[1] may have no tiles
     Deal deal;
-    int segment;            // dx: steps of the first of its two contractions
+    int fine;               // d[2], d[3]: second terms of d[0], d[1]
+    float* partial[3];      // dx, dw, dw_up: the parts' sums, [part][row][col], where parts > 1
     const float* num; const float* den[2];  // dw[i] *= num / den[i]
     const float* dx_scale;                  // dx *= this
     int* status;
 };
 struct Maps {
-    CUtensorMap d[2], w[2], x, dx, dw[2];
+    CUtensorMap d[4], w[2], x, dx, dw[2];
 };
+
+__device__ __forceinline__ float result_scale(const float* num, const float* den)
+{
+    float v = num != nullptr ? __ldg(num) : 1.0f;
+    if (den != nullptr) {
+        const float d = __ldg(den);
+        if (d != 0.0f) v /= d;  // (0: dg was left as it is)
+    }
+    return v;
+}
 
 struct Tile {
     const Kind* kind;
-    int weight, matrix, tm, tn;
+    int weight, matrix, part, tm, tn;
+    int step0, step1;  // of the contraction
 };
 __device__ __forceinline__ bool take_tile(const GradArgs& a, int worker, int workers, int i, Tile& t)
 {
@@ -185,8 +223,13 @@ __device__ __forceinline__ bool take_tile(const GradArgs& a, int worker, int wor
     t.kind = &k;
     t.weight = k.weight;
     const int per = k.tiles_m * k.tiles_n;
-    t.matrix = tile / per;
-    tile -= t.matrix * per;
+    t.matrix = tile / (per * k.parts);
+    tile -= t.matrix * per * k.parts;
+    t.part = tile / per;
+    tile -= t.part * per;
+    const long long steps = static_cast<long long>(k.segments) * k.seg_steps;
+    t.step0 = static_cast<int>(steps * t.part / k.parts);
+    t.step1 = static_cast<int>(steps * (t.part + 1) / k.parts);
     // Raster: groups of 16 row blocks share their column panel in L2.
     constexpr int kGroupM = 16;
     const int group = tile / (kGroupM * k.tiles_n);
@@ -247,7 +290,8 @@ grad_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Grad
         for (int i = 0; alive && take_tile(a, worker, workers, i, t); ++i) {
             const int row = (t.tm * 2 + static_cast<int>(cta_rank)) * kBM;
             const int col = t.tn * kBN + static_cast<int>(cta_rank) * 128;
-            for (int st = 0; st < t.kind->steps; ++st, ++it) {
+            int seg = t.step0 / t.kind->seg_steps, in_seg = t.step0 - seg * t.kind->seg_steps;
+            for (int st = t.step0; st < t.step1; ++st, ++it) {
                 const uint32_t s = it % S, r = it / S;
                 if (!mbar_wait_warp(empty(s), (r & 1u) ^ 1u, abort_flag)) { alive = false; break; }
                 if (elect_one()) {
@@ -255,17 +299,18 @@ grad_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Grad
                     if (cta_rank == 0) mbar_expect_tx(full(s), 2 * kStage);
                     const uint32_t bar = cluster_address(full(s), 0);
                     const uint32_t dst = ring + s * kStage;
-                    // dx contracts over d[0], w[0] and then, for a gated product, d[1], w[1].
-                    const int part = t.weight ? t.matrix : (st >= a.segment ? 1 : 0);
-                    const int k0 = (t.weight || part == 0 ? st : st - a.segment) * kStepK;
-                    const CUtensorMap* ta = &maps.d[part];
-                    const CUtensorMap* tb = t.weight ? &maps.x : &maps.w[part];
+                    // dx: d[0] w[0] (+ d[2] w[0]) + d[1] w[1] (+ d[3] w[1]); dw[i]: d[i]^T x (+ d[i + 2]^T x)
+                    const int term = a.fine ? seg & 1 : 0, which = t.weight ? t.matrix : (a.fine ? seg >> 1 : seg);
+                    const int k0 = in_seg * kStepK;
+                    const CUtensorMap* ta = &maps.d[which + 2 * term];
+                    const CUtensorMap* tb = t.weight ? &maps.x : &maps.w[which];
                     tma_load_2d_pair(dst, ta, bar, t.weight ? row : k0, t.weight ? k0 : row);
                     tma_load_2d_pair(dst + kChunk, ta, bar, t.weight ? row + 64 : k0, t.weight ? k0 : row + 64);
                     tma_load_2d_pair(dst + 2 * kChunk, tb, bar, col, k0);
                     tma_load_2d_pair(dst + 3 * kChunk, tb, bar, col + 64, k0);
                 }
                 __syncwarp();
+                if (++in_seg == t.kind->seg_steps) { in_seg = 0; ++seg; }
             }
         }
     } else if (warp == 1) {
@@ -283,7 +328,7 @@ grad_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Grad
                 const uint32_t idesc = umma_idesc_bf16(2 * kBM, kBN, false, true) | (t.weight ? 1u << 15 : 0u);
                 // 16 elements of the contraction on: 32 bytes of a K-major row, or two 1024-byte atoms
                 const uint32_t step_a = t.weight ? 2048 >> 4 : 32 >> 4, step_b = 2048 >> 4;
-                for (int st = 0; st < t.kind->steps; ++st, ++it) {
+                for (int st = t.step0; st < t.step1; ++st, ++it) {
                     const uint32_t s = it % S, r = it / S;
                     if (!mbar_wait_warp(full(s), r & 1u, abort_flag)) { alive = false; break; }
                     tc_fence_after_sync();
@@ -293,9 +338,9 @@ grad_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Grad
                     if (elect_one()) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            umma_bf16<2>(d_tmem, a_desc + step_a * j, b_desc + step_b * j, idesc, (st | j) != 0 ? 1u : 0u);
+                            umma_bf16<2>(d_tmem, a_desc + step_a * j, b_desc + step_b * j, idesc, (st > t.step0 || j > 0) ? 1u : 0u);
                         umma_commit_2cta(empty(s), 3);
-                        if (st == t.kind->steps - 1) umma_commit_2cta(tm_full(buf), 3);
+                        if (st == t.step1 - 1) umma_commit_2cta(tm_full(buf), 3);
                     }
                     __syncwarp();
                 }
@@ -310,16 +355,9 @@ grad_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Grad
         Tile t;
         for (int i = 0; take_tile(a, worker, workers, i, t); ++i) {
             const uint32_t buf = i & 1u, br = static_cast<uint32_t>(i) >> 1;
-            float alpha = 1.0f;
-            if (t.weight) {
-                if (a.num != nullptr) alpha = __ldg(a.num);
-                if (a.den[t.matrix] != nullptr) {
-                    const float d = __ldg(a.den[t.matrix]);
-                    if (d != 0.0f) alpha /= d;
-                }
-            } else if (a.dx_scale != nullptr) {
-                alpha = __ldg(a.dx_scale);
-            }
+            const bool whole = t.kind->parts == 1;
+            const float alpha = !whole ? 1.0f : (t.weight ? result_scale(a.num, a.den[t.matrix]) : result_scale(a.dx_scale, nullptr));
+            float* partial = a.partial[t.weight ? 1 + t.matrix : 0] + (whole ? 0 : static_cast<size_t>(t.part) * t.kind->rows * t.kind->cols);
             const CUtensorMap* out = t.weight ? &maps.dw[t.matrix] : &maps.dx;
             if (!mbar_wait_warp(tm_full(buf), br & 1u, abort_flag)) break;
             tc_fence_after_sync();
@@ -332,6 +370,15 @@ grad_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Grad
                 uint32_t v[64], h[32];
                 load64(t_addr + c, v);
                 tmem_ld_wait();
+                if (!whole) {
+                    if (row0 + lane < t.kind->rows) {
+                        float* dst = partial + static_cast<size_t>(row0 + lane) * t.kind->cols + col0;
+#pragma unroll
+                        for (int q = 0; q < 16; ++q)  // (cols is a multiple of 32)
+                            if (col0 + 4 * q < t.kind->cols) reinterpret_cast<uint4*>(dst)[q] = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+                    }
+                    continue;
+                }
 #pragma unroll
                 for (int j = 0; j < 32; ++j) h[j] = pack16<false>(__uint_as_float(v[2 * j]) * alpha, __uint_as_float(v[2 * j + 1]) * alpha);
                 const uint32_t stg = stage0 + (chunk_no & 1u) * kStoreStage;
@@ -371,23 +418,93 @@ grad_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Grad
     }
 }
 
-// Pieces of the workspace, each on a 256-byte boundary.
-struct Layout {
-    long long d0 = 0, d1 = 0, w0 = 0, w1 = 0, x = 0, bytes = 0, ld = 0;
+// ------------------------------------------------------------- adding parts
+
+struct SumJob {
+    const float* partial;
+    __nv_bfloat16* out;
+    const float* num; const float* den;
+    long long count;  // elements, a multiple of 32
+    int parts;
 };
-Layout layout(long long m, long long n, long long k, bool gated, bool want_dx, bool want_dw)
+struct SumArgs {
+    SumJob job[3];
+    uint32_t first[4];  // blocks of job i: [first[i], first[i + 1])
+};
+constexpr int kSumThreads = 256, kSumElems = 4;
+
+__global__ void __launch_bounds__(kSumThreads)
+sum_parts_kernel(const __grid_constant__ SumArgs a)
 {
-    Layout l;
-    l.ld = (n + 7) / 8 * 8;
-    auto piece = [&](long long bytes) { const long long at = l.bytes; l.bytes += (bytes + 255) / 256 * 256; return at; };
-    if (gated || n % 8 != 0) l.d0 = piece(m * l.ld * 2);  // (else dy is read as it is)
-    if (gated) l.d1 = piece(m * l.ld * 2);
-    if (want_dx) { l.w0 = piece(n * k * 2); if (gated) l.w1 = piece(n * k * 2); }
-    if (want_dw) l.x = piece(m * k * 2);
-    return l;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const uint32_t b = blockIdx.x;
+    const int i = b < a.first[1] ? 0 : (b < a.first[2] ? 1 : 2);
+    const SumJob& j = a.job[i];
+    const long long at = (static_cast<long long>(b - a.first[i]) * kSumThreads + threadIdx.x) * kSumElems;
+    if (at >= j.count) return;
+    float4 sum = __ldg(reinterpret_cast<const float4*>(j.partial + at));
+#pragma unroll 4
+    for (int p = 1; p < j.parts; ++p) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(j.partial + p * j.count + at));
+        sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+    }
+    const float alpha = result_scale(j.num, j.den);
+    *reinterpret_cast<uint2*>(j.out + at) = make_uint2(pack16<false>(sum.x * alpha, sum.y * alpha), pack16<false>(sum.z * alpha, sum.w * alpha));
 }
 
-bool unaligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
+// -------------------------------------------------------------------- plan
+
+// Everything that follows from the sizes alone: kinds, parts, and the workspace's pieces, each on a 256-byte boundary.
+struct Plan {
+    Kind dx, dw;
+    bool fine = false;
+    long long tiles_dx = 0, tiles_dw = 0;
+    long long d[4] = {}, w[2] = {}, x = 0, partial[3] = {}, bytes = 0, ld = 0;
+};
+constexpr int kPlanWorkers = 74;  // CTA pairs of a B200
+constexpr int kMinPart = 8;       // steps of a part: less would be the time of a tile's start and end
+constexpr int kMinSaving = 24;    // steps (0.28 us each) that pay for the partial sums' way and the third launch
+
+Plan plan(long long m, long long n, long long k, bool gated, bool want_dx, bool want_dw)
+{
+    Plan p;
+    const int matrices = gated ? 2 : 1;
+    const int steps_n = static_cast<int>((n + kStepK - 1) / kStepK), steps_m = static_cast<int>((m + kStepK - 1) / kStepK);
+    const int tn = static_cast<int>((k + kBN - 1) / kBN);
+    p.dx = Kind{0, 1, static_cast<int>(m), static_cast<int>(k), static_cast<int>((m + 255) / 256), tn, matrices, steps_n, 1};
+    p.dw = Kind{1, matrices, static_cast<int>(n), static_cast<int>(k), static_cast<int>((n + 255) / 256), tn, 1, steps_m, 1};
+    // What is decided here does not depend on which gradients are wanted, so their bits do not either.
+    const double tiles_dx = static_cast<double>(p.dx.tiles_m) * tn, tiles_dw = static_cast<double>(matrices) * p.dw.tiles_m * tn;
+    const double load = (tiles_dx * matrices * steps_n + tiles_dw * steps_m) / kPlanWorkers;  // steps of a worker
+    // Two terms for dg and du where twice the steps are a few microseconds, or where there are so few values of them
+    // that the time goes into the weights.
+    p.fine = gated && (2.0 * load <= 24.0 || m * n <= 65536);
+    if (p.fine) {
+        p.dx.segments *= 2;
+        p.dw.segments *= 2;
+    }
+    auto cut = [&](Kind& kind, double tiles) {
+        const double steps = static_cast<double>(kind.segments) * kind.seg_steps, own = tiles * steps / kPlanWorkers;
+        const double part = own > kMinPart ? own : kMinPart;
+        if (steps - part >= kMinSaving) kind.parts = static_cast<int>((steps + part - 1.0) / part);
+    };
+    cut(p.dx, tiles_dx);
+    cut(p.dw, tiles_dw);
+    p.tiles_dx = want_dx ? static_cast<long long>(tiles_dx) * p.dx.parts : 0;
+    p.tiles_dw = want_dw ? static_cast<long long>(tiles_dw) * p.dw.parts : 0;
+
+    p.ld = (n + 7) / 8 * 8;
+    auto piece = [&](long long bytes) { const long long at = p.bytes; p.bytes += (bytes + 255) / 256 * 256; return at; };
+    if (gated || n % 8 != 0) p.d[0] = piece(m * p.ld * 2);  // (else dy is read as it is)
+    if (gated) p.d[1] = piece(m * p.ld * 2);
+    if (p.fine) { p.d[2] = piece(m * p.ld * 2); p.d[3] = piece(m * p.ld * 2); }
+    if (want_dx) { p.w[0] = piece(n * k * 2); if (gated) p.w[1] = piece(n * k * 2); }
+    if (want_dw) p.x = piece(m * k * 2);
+    if (want_dx && p.dx.parts > 1) p.partial[0] = piece(p.dx.parts * m * k * 4);
+    if (want_dw && p.dw.parts > 1) for (int i = 0; i < matrices; ++i) p.partial[1 + i] = piece(p.dw.parts * n * k * 4);
+    return p;
+}
 
 // The launch may begin while the one before it in the stream ends; the kernels wait before they touch memory.
 void allow_overlap(cudaLaunchConfig_t& cfg, cudaStream_t stream, cudaLaunchAttribute (&attr)[1])
@@ -400,11 +517,13 @@ void allow_overlap(cudaLaunchConfig_t& cfg, cudaStream_t stream, cudaLaunchAttri
     count_launch();
 }
 
+bool unaligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
+
 }  // namespace
 
 long long fp4_backward_workspace(long long m, long long n, long long k, bool gated, bool want_dx, bool want_dw)
 {
-    return layout(m, n, k, gated, want_dx, want_dw).bytes;
+    return plan(m, n, k, gated, want_dx, want_dw).bytes;
 }
 
 int setup_fp4_backward(DeviceCtx*)
@@ -416,31 +535,32 @@ int launch_fp4_backward(DeviceCtx* ctx, const Fp4Backward& b, cudaStream_t strea
 {
     using B = __nv_bfloat16;
     const Fp4Problem& p = b.forward;
-    const Layout l = layout(p.m, p.n, p.k, p.gated, b.dx != nullptr, b.dw != nullptr);
+    const Plan l = plan(p.m, p.n, p.k, p.gated, b.dx != nullptr, b.dw != nullptr);
     uint8_t* ws = b.workspace;
     const bool direct = !p.gated && p.n % 8 == 0;  // dy as it is
-    const void* d[2] = {direct ? b.dy : ws + l.d0, ws + l.d1};
+    auto at = [&](long long piece) { return reinterpret_cast<B*>(ws + piece); };
+    const void* d[4] = {direct ? b.dy : ws + l.d[0], ws + l.d[1], ws + l.d[2], ws + l.d[3]};
 
     // ------------------------------------------------------------ preparation
     PrepArgs pa = {};
     long long blocks = 0;
     if (!direct) {
-        pa.gate = GateJob{static_cast<const B*>(b.dy), static_cast<const B*>(b.gate), static_cast<const B*>(b.up),
-                          reinterpret_cast<B*>(ws + l.d0), reinterpret_cast<B*>(ws + l.d1), p.w.tensor_scale, p.w_up.tensor_scale,
+        pa.gate = GateJob{static_cast<const B*>(b.dy), static_cast<const B*>(b.gate), static_cast<const B*>(b.up), at(l.d[0]), at(l.d[1]),
+                          l.fine ? at(l.d[2]) : nullptr, l.fine ? at(l.d[3]) : nullptr, p.w.tensor_scale, p.w_up.tensor_scale,
                           p.m, p.n, p.act, p.n % 8 == 0 && !unaligned16(b.dy) && !unaligned16(b.gate) && !unaligned16(b.up), l.ld};
         const long long units = static_cast<long long>(p.m) * ((p.n + 255) / 256);
         if (units > 0xFFFFFFFFll - 8) return INT4L_ERR_TOO_LARGE;
         blocks = (units + kUnitThreads / 32 - 1) / (kUnitThreads / 32);
     }
     int jobs = 0;
-    auto expand = [&](const Fp4& q, long long at) {
+    auto expand = [&](const Fp4& q, long long piece) {
         pa.first[jobs] = static_cast<uint32_t>(blocks);
-        pa.expand[jobs++] = ExpandJob{q.codes, q.scales, q.tensor_scale, reinterpret_cast<B*>(ws + at), q.rows, q.k};
+        pa.expand[jobs++] = ExpandJob{q.codes, q.scales, q.tensor_scale, at(piece), q.rows, q.k};
         blocks += fp4_expand_blocks(q.rows, q.k);
     };
     if (b.dx) {
-        expand(p.w, l.w0);
-        if (p.gated) expand(p.w_up, l.w1);
+        expand(p.w, l.w[0]);
+        if (p.gated) expand(p.w_up, l.w[1]);
     }
     if (b.dw) expand(p.x, l.x);
     if (blocks > 0x7FFFFFFF) return INT4L_ERR_TOO_LARGE;
@@ -459,19 +579,16 @@ int launch_fp4_backward(DeviceCtx* ctx, const Fp4Backward& b, cudaStream_t strea
     GradArgs a = {};
     Maps maps;
     const int matrices = p.gated ? 2 : 1;
-    const int steps_n = (p.n + kStepK - 1) / kStepK, steps_m = (p.m + kStepK - 1) / kStepK;
-    const Kind dx = {0, 1, p.m, p.k, (p.m + 255) / 256, (p.k + kBN - 1) / kBN, matrices * steps_n};
-    const Kind dw = {1, matrices, p.n, p.k, (p.n + 255) / 256, (p.k + kBN - 1) / kBN, steps_m};
-    const long long tiles_dx = b.dx ? static_cast<long long>(dx.tiles_m) * dx.tiles_n : 0;
-    const long long tiles_dw = b.dw ? static_cast<long long>(matrices) * dw.tiles_m * dw.tiles_n : 0;
-    if (tiles_dx + tiles_dw > (1 << 30)) return INT4L_ERR_TOO_LARGE;
-    const bool dx_first = tiles_dw == 0 || (tiles_dx > 0 && dx.steps >= dw.steps);
-    a.kind[0] = dx_first ? dx : dw;
-    a.kind[1] = dx_first ? dw : dx;
-    a.segment = steps_n;
-    const int workers = tiles_dx + tiles_dw < ctx->max_pairs ? static_cast<int>(tiles_dx + tiles_dw) : ctx->max_pairs;
-    a.deal = deal_tiles(static_cast<int>(dx_first ? tiles_dx : tiles_dw), static_cast<int>(dx_first ? tiles_dw : tiles_dx), a.kind[0].steps,
-                        a.kind[1].steps, workers);
+    if (l.tiles_dx + l.tiles_dw > (1 << 30)) return INT4L_ERR_TOO_LARGE;
+    auto part_steps = [](const Kind& k) { return (k.segments * k.seg_steps + k.parts - 1) / k.parts; };
+    const bool dx_first = l.tiles_dw == 0 || (l.tiles_dx > 0 && part_steps(l.dx) >= part_steps(l.dw));
+    a.kind[0] = dx_first ? l.dx : l.dw;
+    a.kind[1] = dx_first ? l.dw : l.dx;
+    const int workers = l.tiles_dx + l.tiles_dw < ctx->max_pairs ? static_cast<int>(l.tiles_dx + l.tiles_dw) : ctx->max_pairs;
+    a.deal = deal_tiles(static_cast<int>(dx_first ? l.tiles_dx : l.tiles_dw), static_cast<int>(dx_first ? l.tiles_dw : l.tiles_dx),
+                        part_steps(a.kind[0]), part_steps(a.kind[1]), workers);
+    a.fine = l.fine;
+    for (int i = 0; i < 3; ++i) a.partial[i] = reinterpret_cast<float*>(ws + l.partial[i]);
     a.num = p.x.tensor_scale;
     if (p.gated) { a.den[0] = p.w.tensor_scale; a.den[1] = p.w_up.tensor_scale; }
     else a.dx_scale = p.w.tensor_scale;
@@ -483,7 +600,8 @@ int launch_fp4_backward(DeviceCtx* ctx, const Fp4Backward& b, cudaStream_t strea
     };
     for (int i = 0; i < matrices; ++i) {
         map(&maps.d[i], d[i], p.n, p.m, d_pitch, 64);
-        if (b.dx) map(&maps.w[i], ws + (i ? l.w1 : l.w0), p.k, p.n, k_pitch, 64);
+        if (l.fine) map(&maps.d[2 + i], d[2 + i], p.n, p.m, d_pitch, 64);
+        if (b.dx) map(&maps.w[i], ws + l.w[i], p.k, p.n, k_pitch, 64);
         if (b.dw) map(&maps.dw[i], i ? b.dw_up : b.dw, p.k, p.n, k_pitch, 32);
     }
     if (b.dw) map(&maps.x, ws + l.x, p.k, p.m, k_pitch, 64);
@@ -495,6 +613,29 @@ int launch_fp4_backward(DeviceCtx* ctx, const Fp4Backward& b, cudaStream_t strea
     cfg2.dynamicSmemBytes = kSmemBytes;
     allow_overlap(cfg2, stream, attr);
     if (cudaLaunchKernelEx(&cfg2, grad_gemm_kernel, maps, a) != cudaSuccess) { cudaGetLastError(); return INT4L_ERR_CUDA; }
+
+    // ----------------------------------------------------------- adding parts
+    SumArgs sa = {};
+    blocks = 0;
+    jobs = 0;
+    auto add = [&](const Kind& kind, int i, void* out, const float* num, const float* den) {
+        if (kind.parts == 1 || out == nullptr) return;
+        const long long count = static_cast<long long>(kind.rows) * kind.cols;
+        sa.first[jobs] = static_cast<uint32_t>(blocks);
+        sa.job[jobs++] = SumJob{a.partial[i], static_cast<B*>(out), num, den, count, kind.parts};
+        blocks += (count + kSumThreads * kSumElems - 1) / (kSumThreads * kSumElems);
+    };
+    add(l.dx, 0, b.dx, a.dx_scale, nullptr);
+    add(l.dw, 1, b.dw, a.num, a.den[0]);
+    add(l.dw, 2, b.dw_up, a.num, a.den[1]);
+    if (jobs == 0) return INT4L_OK;
+    if (blocks > 0x7FFFFFFF) return INT4L_ERR_TOO_LARGE;
+    for (int i = jobs; i < 4; ++i) sa.first[i] = static_cast<uint32_t>(blocks);
+    cudaLaunchConfig_t cfg3 = {};
+    cfg3.gridDim = dim3(static_cast<unsigned>(blocks), 1, 1);
+    cfg3.blockDim = dim3(kSumThreads, 1, 1);
+    allow_overlap(cfg3, stream, attr);
+    if (cudaLaunchKernelEx(&cfg3, sum_parts_kernel, sa) != cudaSuccess) { cudaGetLastError(); return INT4L_ERR_CUDA; }
     return INT4L_OK;
 }
 

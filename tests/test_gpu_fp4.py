@@ -284,7 +284,9 @@ def test_gated(cuda, fmt, act, m, n, k):
 
 # --------------------------------------------------------------------------------------------- backward
 
-GRAD_SHAPES = [(1, 1, 32), (2, 9, 64), (100, 130, 96), (64, 64, 256), (257, 300, 1056), (1000, 513, 288), (300, 2000, 512)]
+# The last ones: contractions cut into parts (few tiles, long), and large enough that dg and du are single bf16 values.
+GRAD_SHAPES = [(1, 1, 32), (2, 9, 64), (100, 130, 96), (64, 64, 256), (257, 300, 1056), (1000, 513, 288), (300, 2000, 512),
+               (4, 6000, 96), (3, 5001, 160), (5000, 40, 64), (2500, 33, 288), (600, 2000, 2048), (601, 2001, 2080)]
 
 
 def grad_bounds(d, w):
@@ -336,6 +338,18 @@ def test_gated_backward(cuda, fmt, act, m, n, k):
     assert a is None and b is None and torch.equal(only_x, dx)
     none, a, b = L.gated_linear_fp4_backward(dh, gate, up, x, wg, wu, act, need=(False, True))
     assert none is None and torch.equal(a, dwg) and torch.equal(b, dwu)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 200, 96), (7, 6000, 64), (130, 400, 320), (60, 1001, 512)])
+def test_gated_backward_of_small_problems_is_as_good_as_one_rounding(cuda, m, n, k):
+    """Small problems carry dg and du in two terms: an error of 2^-16 in them, so what is left is the result's rounding."""
+    x, wg, wu = (R.matrix(L, r, k, "mxfp4", i, cuda, scale=0.25) for i, r in enumerate((m, n, n)))
+    dh, gate, up = (torch.randn((m, n), device=cuda).to(torch.bfloat16) for _ in range(3))
+    g, u, d = gate.double(), up.double(), dh.double()
+    dg, du = d * u * R.act_slope(g, "silu"), d * R.act(g, "silu")
+    want = (dg @ R.values(wg) + du @ R.values(wu), dg.t() @ R.values(x), du.t() @ R.values(x))
+    for got, w in zip(L.gated_linear_fp4_backward(dh, gate, up, x, wg, wu, "silu"), want):
+        assert (got.double() - w).norm() <= 1.05 * (w.to(torch.bfloat16).double() - w).norm()
 
 
 @pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
