@@ -281,10 +281,10 @@ int int4_linear_fp4_gated_launch_async(const int4_linear_fp4_matrix* x, const in
 
 /* Backward passes, bf16 gradients, with respect to the values the operands stand for.  dx_d (m x k) and
  * the weight gradients (n x k) may be left out with NULL, not all of them.  The workspace is 256-byte
- * aligned device memory of at least int4_linear_fp4_grad_workspace_bytes(...) bytes, free again when the
+ * aligned device memory of at least int4_linear_fp4_grad_workspace_bytes(...) bytes (0: none), free again when the
  * work on the stream is done; calls that can run at the same time need one each.
  *   linear  dx = dy w            dw = dy^T x                     (dy: m x n)
- *   gated   dg = dh up act'(gate), du = dh act(gate), rounded to bf16;
+ *   gated   dg = dh up act'(gate), du = dh act(gate), rounded to bf16 (small problems: to twice its bits);
  *           dx = dg w_gate + du w_up     dw_gate = dg^T x     dw_up = du^T x
  * gate_d and up_d are what the forward pass kept. */
 long long int4_linear_fp4_grad_workspace_bytes(int m, int n, int k, int gated, int want_dx, int want_dw);

@@ -55,7 +55,8 @@ int run_backward(Fp4Backward& b, void* workspace_d, long long workspace_bytes, v
     const Fp4Problem& p = b.forward;
     if (!b.dx && !b.dw) return INT4L_ERR_INVALID_ARG;
     if (misaligned(b.dx, 16) || misaligned(b.dw, 16) || misaligned(b.dw_up, 16) || misaligned(workspace_d, 256)) return INT4L_ERR_MISALIGNED;
-    if (!workspace_d || workspace_bytes < fp4_backward_workspace(p.m, p.n, p.k, p.gated, b.dx != nullptr, b.dw != nullptr)) return INT4L_ERR_INVALID_ARG;
+    const long long need = fp4_backward_workspace(p.m, p.n, p.k, p.gated, b.dx != nullptr, b.dw != nullptr);
+    if (need > 0 && (!workspace_d || workspace_bytes < need)) return INT4L_ERR_INVALID_ARG;
     int rc = INT4L_OK;
     DeviceCtx* ctx = current_ctx(&rc);
     if (!ctx) return rc;

@@ -11,12 +11,15 @@
 // rounding (2.4e-3 in the mean square against 1.7e-3).  Where it costs next to nothing (plan() says when) they are
 // carried as the sum of two bf16 values instead, 16 bits, as contractions of twice the length.
 //
-// Two launches, or three.  The first prepares: dg and du (or dy with a row pitch that TMA takes), and the expansions.  The second
+// Up to three launches.  The first prepares: dg and du (or dy with a row pitch that TMA takes), and the expansions.  The second
 // is all products in one persistent kernel, a CTA pair per 256 x 256 tile (tcgen05.mma kind::f16, cta_group::2), two
 // accumulators in tensor memory so that the epilogue overlaps the next tile:
 //     warp 0      TMA, steps of 64 along the contraction, into 128-byte-swizzled slots
 //     warp 1      UMMA issue (CTA 0 for both)
 //     warps 2-5   epilogue: scale, round to bf16, staged TMA stores
+// For few tokens the second launch expands w and x itself: three groups of four warps take turns at turning a step's codes
+// and scales, loaded into a ring of their own, into the bf16 tile that the UMMA reads.
+//
 // No operand is ever transposed: where the contraction runs down the rows of a matrix (w and x always, dy for
 // dw), its tile is read as it lies and the UMMA takes it MN-major.
 //
@@ -170,14 +173,26 @@ backward_prepare_kernel(const __grid_constant__ PrepArgs a)
 // ---------------------------------------------------------------- products
 
 constexpr int kBM = 128, kBN = 256, kStepK = 64;
-constexpr int kThreads = 32 * 6;
-constexpr int kStages = 6;
 constexpr int kStage = 2 * 128 * 128;          // A and B tile of one CTA, 16 KB each
 constexpr int kChunk = kStepK * 128;           // a box: 64 columns x 64 rows
 constexpr int kStoreStage = 4096;              // per warp and buffer
-constexpr int kNumBarriers = 2 * kStages + 4;
-constexpr int kSmemBytes = 1024 + kStages * kStage + 4 * 2 * kStoreStage + kNumBarriers * 8 + 16;
-static_assert(kSmemBytes <= 232448, "shared memory budget");
+constexpr int kPackedStages = 6;
+constexpr int kGroups = 3;                     // expansion groups of 4 warps, taking turns (2: a tenth slower)
+// (every use of a packed stage by the same group: a wait names a phase by its parity only)
+static_assert(kPackedStages % kGroups == 0, "ring depth and groups");
+constexpr int kPackedCodes = kStepK * 64;      // 64 rows x 128 codes
+constexpr int kPackedStage = kPackedCodes + 1024;  // and the scale tiles of those columns: one (mxfp4) or two (nvfp4)
+
+// kUnpack: the B operand is expanded inside the kernel.
+template <bool kUnpack>
+struct Geo {
+    static constexpr int kThreads = 32 * (kUnpack ? 7 + 4 * kGroups : 6);
+    static constexpr int kStages = kUnpack ? 5 : 6;
+    static constexpr int kPacked = kUnpack ? kPackedStages : 0;
+    static constexpr int kNumBarriers = 2 * kStages + 4 + 2 * kPacked;
+    static constexpr int kSmemBytes = 1024 + kStages * kStage + kPacked * kPackedStage + 4 * 2 * kStoreStage + kNumBarriers * 8 + 16;
+    static_assert(kSmemBytes <= 232448, "shared memory budget");
+};
 
 // One kind of tile: dx (its A operand is K-major), or a weight gradient (`matrices` of them, A MN-major).  A contraction
 // is `segments` runs of `seg_steps` steps, each over operands of its own, cut into `parts`.
@@ -194,11 +209,53 @@ struct GradArgs {
     float* partial[3];      // dx, dw, dw_up: the parts' sums, [part][row][col], where parts > 1
     const float* num; const float* den[2];  // dw[i] *= num / den[i]
     const float* dx_scale;                  // dx *= this
+    // In-kernel expansion: scales and (for a scale of 0) tensor scales of w, w_up, x; rows of w and of x; scale tiles along k.
+    const uint8_t* scales[3]; const float* ts[3];
+    int n, m, ktiles;
     int* status;
 };
 struct Maps {
-    CUtensorMap d[4], w[2], x, dx, dw[2];
+    CUtensorMap d[4], w[2], x, dx, dw[2];  // w, x: the expanded matrices, or their codes
 };
+
+// One arrival of the warp, not before every lane's loads have returned (mbar_arrive_after, for a whole warp).
+__device__ __forceinline__ void mbar_arrive_after_warp(uint32_t bar, uint32_t loaded, int lane)
+{
+    const uint32_t all = __reduce_xor_sync(0xFFFFFFFFu, loaded);
+    if (lane == 0) mbar_arrive_after(bar, all);
+}
+
+// 64 codes of one row and their scales (a word of 4 in nvfp4, 2 bytes in mxfp4) -> 64 bf16, eight 16-byte chunks of a
+// 128-byte-swizzled row.
+template <bool kBlock16>
+__device__ __forceinline__ void expand_row(uint4 lo, uint4 hi, uint32_t scale_word, bool zero, uint32_t row_at, int row)
+{
+    const uint32_t words[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+        const uint32_t byte = (scale_word >> (8 * (kBlock16 ? c / 2 : c / 4))) & 0xFFu;
+        float sc;
+        if constexpr (kBlock16) sc = from_e4m3(byte);
+        else sc = byte == 0xFFu ? __uint_as_float(0x7FFFFFFFu) : __uint_as_float(byte ? byte << 23 : 0x00400000u);
+        if (zero) sc = 0.0f;
+        uint32_t h2[4];
+        asm("{\n\t"
+            ".reg .b8 c0, c1, c2, c3;\n\t"
+            "mov.b32 {c0, c1, c2, c3}, %4;\n\t"
+            "cvt.rn.f16x2.e2m1x2 %0, c0;\n\t"
+            "cvt.rn.f16x2.e2m1x2 %1, c1;\n\t"
+            "cvt.rn.f16x2.e2m1x2 %2, c2;\n\t"
+            "cvt.rn.f16x2.e2m1x2 %3, c3;\n\t"
+            "}\n" : "=r"(h2[0]), "=r"(h2[1]), "=r"(h2[2]), "=r"(h2[3]) : "r"(words[c]));
+        uint32_t out[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h2[b]));
+            out[b] = pack16<false>(v.x * sc, v.y * sc);  // exact
+        }
+        sts128(row_at + ((c ^ (row & 7)) << 4), make_uint4(out[0], out[1], out[2], out[3]));
+    }
+}
 
 __device__ __forceinline__ float result_scale(const float* num, const float* den)
 {
@@ -240,23 +297,28 @@ __device__ __forceinline__ bool take_tile(const GradArgs& a, int worker, int wor
     return true;
 }
 
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+template <bool kUnpack, bool kBlock16>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Geo<kUnpack>::kThreads, 1)
 grad_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GradArgs a)
 {
-    constexpr int S = kStages;
+    using G = Geo<kUnpack>;
+    constexpr int S = G::kStages, P = G::kPacked;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
     uint8_t* gbase = smem_raw + (base - raw);
 
     const uint32_t ring = base;
-    const uint32_t st_base = ring + S * kStage;
+    const uint32_t packed = ring + S * kStage;
+    const uint32_t st_base = packed + P * kPackedStage;
     const uint32_t bar_base = st_base + 4 * 2 * kStoreStage;
     auto full     = [&](int i) { return bar_base + 8u * i; };  // (CTA 0's, for the loads of both)
     auto empty    = [&](int i) { return bar_base + 8u * (S + i); };
     auto tm_full  = [&](int i) { return bar_base + 8u * (2 * S + i); };
     auto tm_empty = [&](int i) { return bar_base + 8u * (2 * S + 2 + i); };
-    const uint32_t misc_off = (bar_base - base) + 8u * kNumBarriers;
+    auto pk_full  = [&](int i) { return bar_base + 8u * (2 * S + 4 + i); };
+    auto pk_empty = [&](int i) { return bar_base + 8u * (2 * S + 4 + P + i); };
+    const uint32_t misc_off = (bar_base - base) + 8u * G::kNumBarriers;
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gbase + misc_off);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + misc_off + 4);
 
@@ -267,8 +329,9 @@ grad_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Grad
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (tid == 0) {
-        for (int i = 0; i < S; ++i) { mbar_init(full(i), 1); mbar_init(empty(i), 1); }
+        for (int i = 0; i < S; ++i) { mbar_init(full(i), kUnpack ? 1 + 2 * 4 : 1); mbar_init(empty(i), 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(tm_full(i), 1); mbar_init(tm_empty(i), 4 * 2); }
+        for (int i = 0; i < P; ++i) { mbar_init(pk_full(i), 1); mbar_init(pk_empty(i), 4); }
         *abort_flag = 0;
         mbar_init_fence();
     }
@@ -296,7 +359,7 @@ grad_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Grad
                 if (!mbar_wait_warp(empty(s), (r & 1u) ^ 1u, abort_flag)) { alive = false; break; }
                 if (elect_one()) {
                     // Both CTAs' loads are counted on CTA 0's barrier (which cannot complete before this announcement).
-                    if (cta_rank == 0) mbar_expect_tx(full(s), 2 * kStage);
+                    if (cta_rank == 0) mbar_expect_tx(full(s), kUnpack ? kStage : 2 * kStage);
                     const uint32_t bar = cluster_address(full(s), 0);
                     const uint32_t dst = ring + s * kStage;
                     // dx: d[0] w[0] (+ d[2] w[0]) + d[1] w[1] (+ d[3] w[1]); dw[i]: d[i]^T x (+ d[i + 2]^T x)
@@ -306,8 +369,10 @@ grad_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Grad
                     const CUtensorMap* tb = t.weight ? &maps.x : &maps.w[which];
                     tma_load_2d_pair(dst, ta, bar, t.weight ? row : k0, t.weight ? k0 : row);
                     tma_load_2d_pair(dst + kChunk, ta, bar, t.weight ? row + 64 : k0, t.weight ? k0 : row + 64);
-                    tma_load_2d_pair(dst + 2 * kChunk, tb, bar, col, k0);
-                    tma_load_2d_pair(dst + 3 * kChunk, tb, bar, col + 64, k0);
+                    if constexpr (!kUnpack) {
+                        tma_load_2d_pair(dst + 2 * kChunk, tb, bar, col, k0);
+                        tma_load_2d_pair(dst + 3 * kChunk, tb, bar, col + 64, k0);
+                    }
                 }
                 __syncwarp();
                 if (++in_seg == t.kind->seg_steps) { in_seg = 0; ++seg; }
@@ -344,6 +409,71 @@ grad_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Grad
                     }
                     __syncwarp();
                 }
+            }
+        }
+        __syncwarp();
+    } else if (kUnpack && warp == 6) {
+        // ------------------------- TMA producer of codes and scales, a ring of its own ahead of the expansion
+        uint32_t it = 0;
+        bool alive = true;
+        Tile t;
+        for (int i = 0; alive && take_tile(a, worker, workers, i, t); ++i) {
+            const int col = t.tn * kBN + static_cast<int>(cta_rank) * 128;
+            int seg = t.step0 / t.kind->seg_steps, in_seg = t.step0 - seg * t.kind->seg_steps;
+            const int per_step = kBlock16 ? 2 : 1;  // scale tiles of 128 columns
+            const int first_tile = col / 128 * per_step;
+            const int tiles = min(per_step, a.ktiles - first_tile);  // (none beyond the matrix: those columns are clipped)
+            for (int st = t.step0; st < t.step1; ++st, ++it) {
+                const uint32_t s = it % (P ? P : 1), r = it / (P ? P : 1);
+                if (!mbar_wait_warp(pk_empty(s), (r & 1u) ^ 1u, abort_flag)) { alive = false; break; }
+                if (elect_one()) {
+                    const int which = t.weight ? 2 : (a.fine ? seg >> 1 : seg);
+                    const int k0 = in_seg * kStepK;
+                    const uint32_t dst = packed + s * kPackedStage;
+                    mbar_expect_tx(pk_full(s), kPackedCodes + (tiles > 0 ? tiles * kScaleTileBytes : 0));
+                    tma_load_2d(dst, t.weight ? &maps.x : &maps.w[which], pk_full(s), col / 2, k0);
+                    if (tiles > 0)
+                        bulk_load(dst + kPackedCodes, a.scales[which] + (static_cast<size_t>(k0 >> 7) * a.ktiles + first_tile) * kScaleTileBytes,
+                                  tiles * kScaleTileBytes, pk_full(s));
+                }
+                __syncwarp();
+                if (++in_seg == t.kind->seg_steps) { in_seg = 0; ++seg; }
+            }
+        }
+    } else if (kUnpack && warp >= 7) {
+        // ------------------- expansion: a thread takes 64 columns (half h) of one of the step's 64 rows
+        const int group = (warp - 7) >> 2, h = ((warp - 7) >> 1) & 1, row = ((warp - 7) & 1) * 32 + lane;
+        uint32_t it = 0;
+        bool alive = true;
+        Tile t;
+        float ts[3];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) ts[i] = a.ts[i] != nullptr ? __ldg(a.ts[i]) : 1.0f;
+        for (int i = 0; alive && take_tile(a, worker, workers, i, t); ++i) {
+            int seg = t.step0 / t.kind->seg_steps, in_seg = t.step0 - seg * t.kind->seg_steps;
+            for (int st = t.step0; st < t.step1; ++st, ++it) {
+                const uint32_t ps = it % (P ? P : 1), pr = it / (P ? P : 1), s = it % S, r = it / S;
+                const int which = t.weight ? 2 : (a.fine ? seg >> 1 : seg);
+                const int k0 = in_seg * kStepK;
+                if (++in_seg == t.kind->seg_steps) { in_seg = 0; ++seg; }
+                if (static_cast<int>(it % kGroups) != group) continue;
+                if (!mbar_wait_warp(pk_full(ps), pr & 1u, abort_flag)) { alive = false; break; }
+                const uint32_t src = packed + ps * kPackedStage;
+                // (64-byte swizzle: 16-byte chunk index XOR (row / 2) % 4)
+                const uint32_t row_at = src + row * 64, x = (row >> 1) & 3;
+                const uint4 lo = lds128(row_at + (((2 * h) ^ x) << 4)), hi = lds128(row_at + (((2 * h + 1) ^ x) << 4));
+                const int rr = (k0 + row) & 127;
+                uint32_t word;
+                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(word) : "r"(src + kPackedCodes + (kBlock16 ? h * kScaleTileBytes : 0) + (rr & 31) * 16 + (rr >> 5) * 4));
+                if (!kBlock16) word >>= 16 * h;
+                mbar_arrive_after_warp(pk_empty(ps), lo.x ^ lo.y ^ lo.z ^ lo.w ^ hi.x ^ hi.y ^ hi.z ^ hi.w ^ word, lane);
+                // Rows beyond the matrix have code 0 (read out of bounds) and no defined scale.
+                const bool zero = k0 + row >= (t.weight ? a.m : a.n) || ts[which] == 0.0f;
+                if (!mbar_wait_warp(empty(s), (r & 1u) ^ 1u, abort_flag)) { alive = false; break; }
+                expand_row<kBlock16>(lo, hi, word, zero, ring + s * kStage + (2 + h) * kChunk + row * 128, row);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(full(s), 0);
             }
         }
         __syncwarp();
@@ -459,10 +589,12 @@ sum_parts_kernel(const __grid_constant__ SumArgs a)
 struct Plan {
     Kind dx, dw;
     bool fine = false;
+    bool unpack = false;  // the products expand w and x themselves
     long long tiles_dx = 0, tiles_dw = 0;
     long long d[4] = {}, w[2] = {}, x = 0, partial[3] = {}, bytes = 0, ld = 0;
 };
 constexpr int kPlanWorkers = 74;  // CTA pairs of a B200
+constexpr int kTileSteps = 6;     // a tile's epilogue, in steps: it runs beside the next tile's steps, and is longer than few of them
 constexpr int kMinPart = 8;       // steps of a part: less would be the time of a tile's start and end
 constexpr int kMinSaving = 24;    // steps (0.28 us each) that pay for the partial sums' way and the third launch
 
@@ -479,15 +611,22 @@ Plan plan(long long m, long long n, long long k, bool gated, bool want_dx, bool 
     const double load = (tiles_dx * matrices * steps_n + tiles_dw * steps_m) / kPlanWorkers;  // steps of a worker
     // Two terms for dg and du where twice the steps are a few microseconds, or where there are so few values of them
     // that the time goes into the weights.
+    // Expanded operands go to memory and come back: four times their bytes, twice, which few tokens do not repay, and
+    // it is a launch of its own.  The in-kernel expansion holds the products below 1.4 PFLOP/s.  Measured, in-kernel
+    // against expanded: mxfp4 64 x 8192 x 4096 49 us and 66, 256 rows 60 and 69, 512 rows 78 and 85, gated 512 rows 152
+    // and 158, 128 x 1024 x 1024 16 and 24; nvfp4 1024 rows 109 and 111; 4096 x 4096 x 8192 403 and 351.
+    p.unpack = m <= 512 || load <= 24.0;
     p.fine = gated && (2.0 * load <= 24.0 || m * n <= 65536);
     if (p.fine) {
         p.dx.segments *= 2;
         p.dw.segments *= 2;
     }
     auto cut = [&](Kind& kind, double tiles) {
-        const double steps = static_cast<double>(kind.segments) * kind.seg_steps, own = tiles * steps / kPlanWorkers;
-        const double part = own > kMinPart ? own : kMinPart;
-        if (steps - part >= kMinSaving) kind.parts = static_cast<int>((steps + part - 1.0) / part);
+        // (no more parts than workers: one item too many would double the time)
+        const int steps = kind.segments * kind.seg_steps;
+        int parts = tiles < kPlanWorkers ? static_cast<int>(kPlanWorkers / tiles) : 1;
+        if (parts > steps / kMinPart) parts = steps / kMinPart;
+        if (parts > 1 && steps - steps / parts >= kMinSaving) kind.parts = parts;
     };
     cut(p.dx, tiles_dx);
     cut(p.dw, tiles_dw);
@@ -499,8 +638,8 @@ Plan plan(long long m, long long n, long long k, bool gated, bool want_dx, bool 
     if (gated || n % 8 != 0) p.d[0] = piece(m * p.ld * 2);  // (else dy is read as it is)
     if (gated) p.d[1] = piece(m * p.ld * 2);
     if (p.fine) { p.d[2] = piece(m * p.ld * 2); p.d[3] = piece(m * p.ld * 2); }
-    if (want_dx) { p.w[0] = piece(n * k * 2); if (gated) p.w[1] = piece(n * k * 2); }
-    if (want_dw) p.x = piece(m * k * 2);
+    if (want_dx && !p.unpack) { p.w[0] = piece(n * k * 2); if (gated) p.w[1] = piece(n * k * 2); }
+    if (want_dw && !p.unpack) p.x = piece(m * k * 2);
     if (want_dx && p.dx.parts > 1) p.partial[0] = piece(p.dx.parts * m * k * 4);
     if (want_dw && p.dw.parts > 1) for (int i = 0; i < matrices; ++i) p.partial[1 + i] = piece(p.dw.parts * n * k * 4);
     return p;
@@ -528,7 +667,11 @@ long long fp4_backward_workspace(long long m, long long n, long long k, bool gat
 
 int setup_fp4_backward(DeviceCtx*)
 {
-    return cudaFuncSetAttribute(grad_gemm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) == cudaSuccess ? INT4L_OK : INT4L_ERR_CUDA;
+    const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
+    const bool ok = cudaFuncSetAttribute(grad_gemm_kernel<false, false>, attr, Geo<false>::kSmemBytes) == cudaSuccess &&
+                    cudaFuncSetAttribute(grad_gemm_kernel<true, false>, attr, Geo<true>::kSmemBytes) == cudaSuccess &&
+                    cudaFuncSetAttribute(grad_gemm_kernel<true, true>, attr, Geo<true>::kSmemBytes) == cudaSuccess;
+    return ok ? INT4L_OK : INT4L_ERR_CUDA;
 }
 
 int launch_fp4_backward(DeviceCtx* ctx, const Fp4Backward& b, cudaStream_t stream)
@@ -558,21 +701,23 @@ int launch_fp4_backward(DeviceCtx* ctx, const Fp4Backward& b, cudaStream_t strea
         pa.expand[jobs++] = ExpandJob{q.codes, q.scales, q.tensor_scale, at(piece), q.rows, q.k};
         blocks += fp4_expand_blocks(q.rows, q.k);
     };
-    if (b.dx) {
+    if (b.dx && !l.unpack) {
         expand(p.w, l.w[0]);
         if (p.gated) expand(p.w_up, l.w[1]);
     }
-    if (b.dw) expand(p.x, l.x);
+    if (b.dw && !l.unpack) expand(p.x, l.x);
     if (blocks > 0x7FFFFFFF) return INT4L_ERR_TOO_LARGE;
     for (int i = jobs; i < 4; ++i) pa.first[i] = static_cast<uint32_t>(blocks);
-    cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
-    cfg.gridDim = dim3(static_cast<unsigned>(blocks), 1, 1);
-    cfg.blockDim = dim3(kUnitThreads, 1, 1);
-    allow_overlap(cfg, stream, attr);
-    if (cudaLaunchKernelEx(&cfg, p.x.block16 ? backward_prepare_kernel<true> : backward_prepare_kernel<false>, pa) != cudaSuccess) {
-        cudaGetLastError();
-        return INT4L_ERR_CUDA;
+    if (blocks > 0) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(static_cast<unsigned>(blocks), 1, 1);
+        cfg.blockDim = dim3(kUnitThreads, 1, 1);
+        allow_overlap(cfg, stream, attr);
+        if (cudaLaunchKernelEx(&cfg, p.x.block16 ? backward_prepare_kernel<true> : backward_prepare_kernel<false>, pa) != cudaSuccess) {
+            cudaGetLastError();
+            return INT4L_ERR_CUDA;
+        }
     }
 
     // --------------------------------------------------------------- products
@@ -581,38 +726,49 @@ int launch_fp4_backward(DeviceCtx* ctx, const Fp4Backward& b, cudaStream_t strea
     const int matrices = p.gated ? 2 : 1;
     if (l.tiles_dx + l.tiles_dw > (1 << 30)) return INT4L_ERR_TOO_LARGE;
     auto part_steps = [](const Kind& k) { return (k.segments * k.seg_steps + k.parts - 1) / k.parts; };
+    auto tile_cost = [&](const Kind& k) { return part_steps(k) > kTileSteps ? part_steps(k) : kTileSteps; };
     const bool dx_first = l.tiles_dw == 0 || (l.tiles_dx > 0 && part_steps(l.dx) >= part_steps(l.dw));
     a.kind[0] = dx_first ? l.dx : l.dw;
     a.kind[1] = dx_first ? l.dw : l.dx;
     const int workers = l.tiles_dx + l.tiles_dw < ctx->max_pairs ? static_cast<int>(l.tiles_dx + l.tiles_dw) : ctx->max_pairs;
     a.deal = deal_tiles(static_cast<int>(dx_first ? l.tiles_dx : l.tiles_dw), static_cast<int>(dx_first ? l.tiles_dw : l.tiles_dx),
-                        part_steps(a.kind[0]), part_steps(a.kind[1]), workers);
+                        tile_cost(a.kind[0]), tile_cost(a.kind[1]), workers);
     a.fine = l.fine;
     for (int i = 0; i < 3; ++i) a.partial[i] = reinterpret_cast<float*>(ws + l.partial[i]);
     a.num = p.x.tensor_scale;
     if (p.gated) { a.den[0] = p.w.tensor_scale; a.den[1] = p.w_up.tensor_scale; }
     else a.dx_scale = p.w.tensor_scale;
+    const Fp4* operands[3] = {&p.w, &p.w_up, &p.x};
+    for (int i = 0; i < 3; ++i) { a.scales[i] = operands[i]->scales; a.ts[i] = operands[i]->tensor_scale; }
+    a.n = p.n; a.m = p.m;
+    a.ktiles = fp4_ktiles(p.k, p.x.block16);
     a.status = ctx->status_dev;
     const uint64_t d_pitch = direct ? static_cast<uint64_t>(p.n) * 2 : static_cast<uint64_t>(l.ld) * 2, k_pitch = static_cast<uint64_t>(p.k) * 2;
     int rc = INT4L_OK;
     auto map = [&](CUtensorMap* out, const void* at, int cols, int rows, uint64_t pitch, int box_rows) {
         if (rc == INT4L_OK) rc = encode_tensor_map_2d(ctx, out, at, 2, cols, rows, pitch, 64, box_rows, true);
     };
+    auto codes = [&](CUtensorMap* out, const Fp4& q) {
+        if (rc == INT4L_OK) rc = encode_tensor_map_2d(ctx, out, q.codes, 1, static_cast<uint64_t>(q.k) / 2, q.rows, static_cast<uint64_t>(q.k) / 2, 64, kStepK, false, true);
+    };
     for (int i = 0; i < matrices; ++i) {
         map(&maps.d[i], d[i], p.n, p.m, d_pitch, 64);
         if (l.fine) map(&maps.d[2 + i], d[2 + i], p.n, p.m, d_pitch, 64);
-        if (b.dx) map(&maps.w[i], ws + l.w[i], p.k, p.n, k_pitch, 64);
+        if (b.dx && l.unpack) codes(&maps.w[i], i ? p.w_up : p.w);
+        else if (b.dx) map(&maps.w[i], ws + l.w[i], p.k, p.n, k_pitch, 64);
         if (b.dw) map(&maps.dw[i], i ? b.dw_up : b.dw, p.k, p.n, k_pitch, 32);
     }
-    if (b.dw) map(&maps.x, ws + l.x, p.k, p.m, k_pitch, 64);
+    if (b.dw && l.unpack) codes(&maps.x, p.x);
+    else if (b.dw) map(&maps.x, ws + l.x, p.k, p.m, k_pitch, 64);
     if (b.dx) map(&maps.dx, b.dx, p.k, p.m, k_pitch, 32);
     if (rc != INT4L_OK) return rc;
     cudaLaunchConfig_t cfg2 = {};
     cfg2.gridDim = dim3(workers * 2, 1, 1);
-    cfg2.blockDim = dim3(kThreads, 1, 1);
-    cfg2.dynamicSmemBytes = kSmemBytes;
+    cfg2.blockDim = dim3(l.unpack ? Geo<true>::kThreads : Geo<false>::kThreads, 1, 1);
+    cfg2.dynamicSmemBytes = l.unpack ? Geo<true>::kSmemBytes : Geo<false>::kSmemBytes;
     allow_overlap(cfg2, stream, attr);
-    if (cudaLaunchKernelEx(&cfg2, grad_gemm_kernel, maps, a) != cudaSuccess) { cudaGetLastError(); return INT4L_ERR_CUDA; }
+    const auto kernel = !l.unpack ? grad_gemm_kernel<false, false> : (p.x.block16 ? grad_gemm_kernel<true, true> : grad_gemm_kernel<true, false>);
+    if (cudaLaunchKernelEx(&cfg2, kernel, maps, a) != cudaSuccess) { cudaGetLastError(); return INT4L_ERR_CUDA; }
 
     // ----------------------------------------------------------- adding parts
     SumArgs sa = {};

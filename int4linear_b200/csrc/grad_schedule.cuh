@@ -1,8 +1,9 @@
 // Dealing out the tiles of a backward pass (gemm_grad.cu) to the workers of a persistent kernel (host + device).
 //
 // There are two kinds of tile, kind 0 with the longer contraction.  Kind 0 goes round-robin; a worker that got one
-// tile fewer than others first takes `extra` tiles of kind 1, about as long as one of kind 0 together; the rest of
-// kind 1 goes round-robin.  Every role of the kernel enumerates the same list, so the roles agree without talking.
+// tile fewer than others first takes `extra` tiles of kind 1; the rest of kind 1 goes round-robin.  `extra` is the
+// number that ends the busiest worker soonest.  Every role of the kernel enumerates the same list, so the roles agree
+// without talking.
 #pragma once
 
 #ifndef __CUDACC__
@@ -39,13 +40,28 @@ struct Deal {
     }
 };
 
-// steps0 >= steps1: lengths of the two kinds' contractions.
-inline Deal deal_tiles(int tiles0, int tiles1, int steps0, int steps1, int workers)
+// cost0 >= cost1: time of a tile of either kind, in any unit.
+inline Deal deal_tiles(int tiles0, int tiles1, int cost0, int cost1, int workers)
 {
     Deal d;
     d.tiles[0] = tiles0;
     d.tiles[1] = tiles1;
-    d.extra = tiles0 % workers == 0 ? 0 : (steps0 + steps1 / 2) / steps1;
+    const int full = tiles0 % workers;
+    if (full == 0) return d;
+    const long long few = workers - full, rounds0 = tiles0 / workers;
+    long long best = -1;
+    for (long long extra = 0; extra <= cost0 / cost1 + 1; ++extra) {
+        const long long dealt = few * extra < tiles1 ? few * extra : tiles1, rest = tiles1 - dealt;
+        // The rest goes to workers 0, 1, ..., so those with one tile more of kind 0 (they come first) get the odd ones.
+        const long long hi = (rounds0 + 1) * cost0 + (rest + workers - 1) / workers * cost1;
+        const long long odd = rest % workers > full ? 1 : 0;
+        const long long lo = rounds0 * cost0 + ((dealt + few - 1) / few + rest / workers + odd) * cost1;
+        const long long end = hi > lo ? hi : lo;
+        if (best < 0 || end < best) {
+            best = end;
+            d.extra = static_cast<int>(extra);
+        }
+    }
     return d;
 }
 

@@ -359,7 +359,7 @@ def gated_linear_fp4_backward(grad_h, gate, up, x: Fp4Matrix, w_gate: Fp4Matrix,
     """(dX, dWg, dWu) of gated_linear_fp4 in bfloat16, with respect to the values the operands stand for.
 
     gate, up: the products kept by the forward pass, bfloat16 [m, n] like grad_h.
-    dG = dH up act'(gate) and dU = dH act(gate) are rounded to bfloat16; dX = dG Wg + dU Wu, dWg = dG^T X, dWu = dU^T X.
+    dG = dH up act'(gate) and dU = dH act(gate) are rounded to bfloat16 (small problems: to twice its bits); dX = dG Wg + dU Wu, dWg = dG^T X, dWu = dU^T X.
     `need` = (input, weights) leaves gradients out (None in their place)."""
     import torch
     m, n = _check_operands(x, w_gate, w_up)

@@ -72,12 +72,14 @@ def test_c_entry_points_refuse_bad_arguments():
     assert g(ref(ok), ref(ok), ref(ok), 0, BASE, BASE, None, 0, None) == 1     # gate without up
     assert g(ref(ok), ref(ok), ref(ok), 0, BASE, BASE + 2, BASE, 0, None) == 3
     b = lib.int4_linear_fp4_grad_async
-    need = lib.int4_linear_fp4_grad_workspace_bytes(8, 8, 64, 0, 1, 1)
+    assert lib.int4_linear_fp4_grad_workspace_bytes(8, 8, 64, 0, 1, 1) == 0  # nothing to lay out anew
+    odd = matrix(rows=9)
+    need = lib.int4_linear_fp4_grad_workspace_bytes(8, 9, 64, 0, 1, 1)
     assert need > 0 and need % 256 == 0
     assert b(None, ref(ok), ref(ok), BASE, BASE, BASE, need, None) == 1
     assert b(BASE, ref(ok), ref(ok), None, None, BASE, need, None) == 1       # nothing wanted
-    assert b(BASE, ref(ok), ref(ok), BASE, BASE, BASE, need - 1, None) == 1   # workspace too small
-    assert b(BASE, ref(ok), ref(ok), BASE, BASE, None, need, None) == 1
+    assert b(BASE, ref(ok), ref(odd), BASE, BASE, BASE, need - 1, None) == 1  # workspace too small
+    assert b(BASE, ref(ok), ref(odd), BASE, BASE, None, need, None) == 1
     assert b(BASE, ref(ok), ref(ok), BASE, BASE, BASE + 128, big, None) == 3
     assert b(BASE + 2, ref(ok), ref(ok), BASE, BASE, BASE, need, None) == 3   # n % 8 == 0: 16-byte rows
     h = lib.int4_linear_fp4_gated_grad_async
