@@ -206,40 +206,46 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
         if (cta_rank == 0) {
             // ----------------------------------------------------- UMMA issuer
             // The warp walks the ring together and one elected thread issues.
-            uint32_t it = 0, local_tile = 0;
+            uint32_t s = 0, phase = 0, local_tile = 0;
             bool alive = true;
+            const uint32_t codes_low = umma_desc_sw128_low(ring), scales_low = scale_tile_low(ring + G::kCodeBytes);
+            const uint32_t scale_cols = tmem_base + kScaleCol;
+            const int last_count = (a.k - (steps - 1) * kStepK + 63) / 64;  // UMMAs of the last step
+            // One step: scales, then `count` UMMAs (a constant but in the last step).
+            auto issue = [&](int count, bool first) {
+                const uint32_t x_low = codes_low + s * (G::kStage / 16), w_low = x_low + 128 * kStepBytes / 16;
+                const uint32_t sfa_low = scales_low + s * (G::kStage / 16), sfb_low = sfa_low + G::kScaleBytesA / 16;
+                const uint32_t sfa = scale_cols + s * G::kScaleCols, sfb = sfa + 4 * G::kTilesK;
+#pragma unroll
+                for (int t = 0; t < G::kTilesK; ++t) {
+                    tmem_copy_scales<2>(sfa + 4 * t, sfa_low + t * (kScaleTileBytes / 16));
+                    tmem_copy_scales<2>(sfb + 8 * t, sfb_low + t * (kScaleTileBytes / 16));
+                    tmem_copy_scales<2>(sfb + 8 * t + 4, sfb_low + (G::kScaleBytesA + t * kScaleTileBytes) / 16);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (j >= count) break;
+                    const int t = kBlock16 ? j : j >> 1;
+                    const uint32_t idesc = umma_idesc_fp4(2 * kBM, kBN, !kBlock16, kBlock16 ? 0u : 2u * (j & 1));
+                    umma_fp4<2, kBlock16>(tmem_base, x_low + 2 * j, w_low + 2 * j, idesc, sfa + 4 * t, sfb + 8 * t, (j > 0 || !first) ? 1u : 0u);
+                }
+                umma_commit_2cta(empty(s), 3);
+            };
             for (int tile = worker; alive && tile < num_tiles; tile += workers, ++local_tile) {
                 if (local_tile > 0 && !mbar_wait_warp(acc_free, (local_tile - 1) & 1u, abort_flag)) break;
-                tc_fence_after_sync();
-                for (int kb = 0; kb < steps; ++kb, ++it) {
-                    const uint32_t s = it % S, r = it / S;
-                    if (!mbar_wait_warp(full(s), r & 1u, abort_flag)) { alive = false; break; }
+                for (int kb = 0; kb < steps; ++kb) {
+                    if (!mbar_wait_warp(full(s), phase, abort_flag)) { alive = false; break; }
                     tc_fence_after_sync();
-                    const uint32_t a_addr = ring + s * G::kStage;
-                    const uint32_t sfa_smem = a_addr + G::kCodeBytes, sfb_smem = sfa_smem + G::kScaleBytesA;
-                    const uint32_t sfa = tmem_base + kScaleCol + s * G::kScaleCols;
-                    const uint32_t sfb = sfa + 4 * G::kTilesK;
-                    const int umma_count = min(4, (a.k - kb * kStepK + 63) / 64);
-                    const uint64_t a_desc = umma_desc_sw128(a_addr);
-                    const uint64_t b_desc = umma_desc_sw128(a_addr + 128 * kStepBytes);
                     if (elect_one()) {
-#pragma unroll
-                        for (int t = 0; t < G::kTilesK; ++t) {
-                            tmem_copy_scales<2>(sfa + 4 * t, scale_tile_desc(sfa_smem + t * kScaleTileBytes));
-                            tmem_copy_scales<2>(sfb + 8 * t, scale_tile_desc(sfb_smem + t * kScaleTileBytes));
-                            tmem_copy_scales<2>(sfb + 8 * t + 4, scale_tile_desc(sfb_smem + G::kScaleBytesA + t * kScaleTileBytes));
+                        if (kb < steps - 1) {
+                            issue(4, kb == 0);
+                        } else {
+                            issue(last_count, kb == 0);
+                            umma_commit_2cta(acc_full, 3);
                         }
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            if (j >= umma_count) break;
-                            const int t = kBlock16 ? j : j >> 1;
-                            const uint32_t idesc = umma_idesc_fp4(2 * kBM, kBN, !kBlock16, kBlock16 ? 0u : 2u * (j & 1));
-                            umma_fp4<2, kBlock16>(tmem_base, a_desc + 2u * j, b_desc + 2u * j, idesc, sfa + 4 * t, sfb + 8 * t, (kb | j) != 0 ? 1u : 0u);
-                        }
-                        umma_commit_2cta(empty(s), 3);
-                        if (kb == steps - 1) umma_commit_2cta(acc_full, 3);
                     }
                     __syncwarp();
+                    if (++s == S) { s = 0; phase ^= 1u; }
                 }
             }
         }

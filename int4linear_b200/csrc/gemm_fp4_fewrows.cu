@@ -170,11 +170,11 @@ gemm_fp4_fewrows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
             const uint32_t sf = scale_cols + s * G::kScaleCols;
             const uint32_t sfx = sf + 4 * G::kTilesK * G::kW;
             const int umma_count = min(4, (a.k - kb * kStepK + 63) / 64);
-            const uint64_t x_desc = umma_desc_sw128(at + G::kOffX);
+            const uint32_t x_low = umma_desc_sw128_low(at + G::kOffX), w_low = umma_desc_sw128_low(at), scales_low = scale_tile_low(at + G::kOffScales);
             if (elect_one()) {
 #pragma unroll
                 for (int t = 0; t < (G::kW + 1) * G::kTilesK; ++t)
-                    tmem_copy_scales<1>(sf + 4 * t, scale_tile_desc(at + G::kOffScales + t * kScaleTileBytes));
+                    tmem_copy_scales<1>(sf + 4 * t, scales_low + t * (kScaleTileBytes / 16));
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     if (j >= umma_count) break;
@@ -182,7 +182,7 @@ gemm_fp4_fewrows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
                     const uint32_t idesc = umma_idesc_fp4(kRows, 0, !kBlock16, kBlock16 ? 0u : 2u * (j & 1)) | (static_cast<uint32_t>(a.n_pad >> 3) << 17);
 #pragma unroll
                     for (int i = 0; i < G::kW; ++i)
-                        umma_fp4<1, kBlock16>(tmem_base + i * a.n_pad, umma_desc_sw128(at + i * G::kCodesW) + 2u * j, x_desc + 2u * j, idesc,
+                        umma_fp4<1, kBlock16>(tmem_base + i * a.n_pad, w_low + i * (G::kCodesW / 16) + 2 * j, x_low + 2 * j, idesc,
                                               sf + 4 * (i * G::kTilesK + t), sfx + 4 * t, (kb > kb0 || j > 0) ? 1u : 0u);
                 }
                 umma_commit(empty(s));

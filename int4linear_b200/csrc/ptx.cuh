@@ -361,17 +361,25 @@ __host__ __device__ constexpr uint32_t umma_idesc_fp4(int m, int n, bool ue8m0, 
 // D[tmem] (+)= (A[smem] scaled) * (B[smem] scaled)^T, K = 64, scales in tensor memory (a row's scale word in
 // lane row % 32, column row / 32, the 32 lanes repeated in all four quarters).  Issued by ONE thread.
 // kBlock16: nvfp4 (a ue4m3 scale per 16 elements), else mxfp4 (a ue8m0 scale per 32).
+// The operand descriptors are those of umma_desc_sw128, given by their low words (address and leading offset): the high
+// word is a constant, and the issuing warp, whose instructions bound the step, adds 32 bits instead of 64.
+__device__ __forceinline__ uint32_t umma_desc_sw128_low(uint32_t smem_addr) { return ((smem_addr & 0x3FFFFu) >> 4) | (1u << 16); }
+constexpr uint32_t kUmmaDescSw128High = (1024u >> 4) | (1u << 14) | (2u << 29);
+
 template <int kCtaGroup, bool kBlock16>
-__device__ __forceinline__ void umma_fp4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+__device__ __forceinline__ void umma_fp4(uint32_t d_tmem, uint32_t a_low, uint32_t b_low, uint32_t idesc,
                                          uint32_t sfa_tmem, uint32_t sfb_tmem, uint32_t accumulate) {
 #define I4L_UMMA_FP4(GROUP, KIND)                                                                        \
     asm volatile(                                                                                        \
         "{\n\t"                                                                                          \
         ".reg .pred p;\n\t"                                                                              \
+        ".reg .b64 da, db;\n\t"                                                                          \
+        "mov.b64 da, {%1, %7};\n\t"                                                                      \
+        "mov.b64 db, {%2, %7};\n\t"                                                                      \
         "setp.ne.b32 p, %6, 0;\n\t"                                                                      \
-        "tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, [%4], [%5], p;\n\t"           \
-        "}\n" ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem),         \
-        "r"(accumulate) : "memory")
+        "tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], da, db, %3, [%4], [%5], p;\n\t"           \
+        "}\n" ::"r"(d_tmem), "r"(a_low), "r"(b_low), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem),           \
+        "r"(accumulate), "r"(kUmmaDescSw128High) : "memory")
     if constexpr (kCtaGroup == 1) {
         if constexpr (kBlock16) I4L_UMMA_FP4("1", "mxf4nvf4.block_scale.scale_vec::4X");
         else I4L_UMMA_FP4("1", "mxf4.block_scale.scale_vec::2X");
@@ -382,23 +390,18 @@ __device__ __forceinline__ void umma_fp4(uint32_t d_tmem, uint64_t a_desc, uint6
 #undef I4L_UMMA_FP4
 }
 
-// Shared-memory descriptor of one 512-byte scale tile (32 rows of 16 bytes, no swizzle: 8-row groups of
-// 128 bytes that follow one another) for tcgen05.cp 32x128b.
-__device__ __forceinline__ uint64_t scale_tile_desc(uint32_t smem_addr) {
-    uint64_t d = 0;
-    d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
-    d |= static_cast<uint64_t>(128 >> 4) << 32;
-    d |= static_cast<uint64_t>(1) << 46;
-    return d;
-}
-// Copies one scale tile into 4 columns of tensor memory (repeated in the four lane quarters).  Issued by the
-// thread that issues the UMMAs reading it: copies and UMMAs of one thread are executed in order.
+// Copies one 512-byte scale tile (32 rows of 16 bytes, no swizzle: 8-row groups of 128 bytes that follow one another;
+// tcgen05.cp 32x128b) into 4 columns of tensor memory, repeated in the four lane quarters.  `low` is the tile's
+// shared-memory address >> 4.  Issued by the thread that issues the UMMAs reading it: copies and UMMAs of one thread are
+// executed in order.
+__device__ __forceinline__ uint32_t scale_tile_low(uint32_t smem_addr) { return (smem_addr & 0x3FFFFu) >> 4; }
 template <int kCtaGroup>
-__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint32_t low) {
+    constexpr uint32_t kHigh = (128u >> 4) | (1u << 14);
     if constexpr (kCtaGroup == 1)
-        asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+        asm volatile("{\n\t.reg .b64 d;\n\tmov.b64 d, {%1, %2};\n\ttcgen05.cp.cta_group::1.32x128b.warpx4 [%0], d;\n\t}\n" ::"r"(taddr), "r"(low), "r"(kHigh) : "memory");
     else
-        asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+        asm volatile("{\n\t.reg .b64 d;\n\tmov.b64 d, {%1, %2};\n\ttcgen05.cp.cta_group::2.32x128b.warpx4 [%0], d;\n\t}\n" ::"r"(taddr), "r"(low), "r"(kHigh) : "memory");
 }
 
 // Instruction descriptor for kind::f16 with bfloat16 operands and an fp32 accumulator.
