@@ -235,6 +235,7 @@ int int4_linear_unpack_i32(const void* src_d, int* dst_d, int rows, int cols, vo
  */
 #define INT4L_FP4_MX 0
 #define INT4L_FP4_NV 1
+#define INT4L_FP4_MAX_EXTENT (1 << 26)  /* rows and k; beyond: INT4L_ERR_TOO_LARGE */
 
 #define INT4L_TYPE_BF16 0
 #define INT4L_TYPE_F16  1

@@ -14,6 +14,7 @@ int take_matrix(const int4_linear_fp4_matrix* q, Fp4* out)
     if (q->format != INT4L_FP4_MX && q->format != INT4L_FP4_NV) return INT4L_ERR_INVALID_ARG;
     if (q->format == INT4L_FP4_MX && q->tensor_scale) return INT4L_ERR_INVALID_ARG;
     if (q->k % 32 != 0) return INT4L_ERR_UNSUPPORTED;
+    if (q->rows > INT4L_FP4_MAX_EXTENT || q->k > INT4L_FP4_MAX_EXTENT) return INT4L_ERR_TOO_LARGE;
     if (misaligned(q->codes, 16) || misaligned(q->scales, 16) || misaligned(q->tensor_scale, 4)) return INT4L_ERR_MISALIGNED;
     out->codes = static_cast<const uint8_t*>(q->codes);
     out->scales = static_cast<const uint8_t*>(q->scales);

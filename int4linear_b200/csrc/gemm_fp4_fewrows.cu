@@ -10,9 +10,9 @@
 //
 // Bound: HBM.  A CTA's shared memory is kept to a half or a third of an SM's, so that the loads of one CTA cover the
 // start and the reduction of another.  Tensor memory is shared between the CTAs of an SM too, and its allocation
-// waits while there is none: a CTA that waits could be one that others wait for.  Therefore every launch takes at
-// least 448 bytes of shared memory per column, which keeps any mixture of resident CTAs within the 512 columns
-// (228 KB / 448 = 521, and allocations are multiples of 128): no allocation ever waits.
+// waits while there is none.  Every launch takes at least 448 bytes of shared memory per column, which keeps any
+// mixture of resident CTAs of this kernel within the 512 columns (228 KB / 448 = 521, and allocations are multiples of
+// 128), so none of its allocations waits for another.
 //     warp 0      TMA (as in gemm_fp4.cu)
 //     warp 1      tcgen05.cp of the scales and UMMAs
 //     all 4       epilogue
@@ -195,6 +195,12 @@ gemm_fp4_fewrows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
     __syncwarp();
 
     // ---------------------------------------------------------------- epilogue
+    // A bias is fetched while the products run: of the thread's column, or of the four it sums up below.
+    auto bias_of = [&](int col) { return (!kGated && a.bias != nullptr && col < a.n) ? __ldg(a.bias + col) : 0.0f; };
+    const int bias_col = tile * kRows + (split == 1 ? tid : 4 * lane);
+    float bias[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) bias[e] = (e == 0 || split > 1) ? bias_of(bias_col + e) : 0.0f;
     const bool ok = mbar_wait_warp(acc_full, 0, abort_flag);
     tc_fence_after_sync();
     const float ts_x = a.ts_x != nullptr ? __ldg(a.ts_x) : 1.0f;
@@ -212,12 +218,10 @@ gemm_fp4_fewrows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
             a.y[at] = bits(fmaf(acc, alpha, bias));
         }
     };
-    auto bias_of = [&](int col) { return (!kGated && a.bias != nullptr && col < a.n) ? __ldg(a.bias + col) : 0.0f; };
     const uint32_t lanes = tmem_base + (static_cast<uint32_t>(warp * 32) << 16);
     // All UMMAs of this CTA are done with the ring (acc_full): it takes the partial sums, [x row][w row] floats.
     if (ok) {
         const int col = tile * kRows + tid;
-        const float bias = split == 1 ? bias_of(col) : 0.0f;
 #pragma unroll 1
         for (int c = 0; c < m; c += 16) {
             uint32_t v[G::kW][16];
@@ -228,7 +232,7 @@ gemm_fp4_fewrows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
                 if (col < a.n) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
-                        if (c + e < m) put(c + e, col, __uint_as_float(v[0][e]), __uint_as_float(v[G::kW - 1][e]), bias);
+                        if (c + e < m) put(c + e, col, __uint_as_float(v[0][e]), __uint_as_float(v[G::kW - 1][e]), bias[0]);
                 }
             } else {
 #pragma unroll
@@ -238,16 +242,25 @@ gemm_fp4_fewrows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
             }
         }
     }
+    // Tensor memory goes back before any wait for another CTA: whoever holds it never waits for a CTA that might wait
+    // for it.
     tc_fence_before_sync();
+    __syncthreads();
+    if (*abort_flag) {
+        if (tid == 0) atomicExch(a.status, INT4L_ERR_DEVICE_TIMEOUT);
+        for (int i = 0; i < 100; ++i) __nanosleep(1000);  // copies and UMMAs in flight end
+        __syncthreads();
+    }
+    if (warp == 1) {
+        tc_fence_after_sync();
+        tmem_dealloc<1>(tmem_base, a.cols);
+    }
     __syncwarp();
     if (split > 1) {
         cluster_sync_all();
         // Rows of x are dealt out to the warps of the cluster, four columns to a lane; each value is summed in the
         // order of k.
         const int col = tile * kRows + 4 * lane;
-        float bias[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) bias[e] = bias_of(col + e);
         if (ok) {
 #pragma unroll 2
             for (int i = warp * split + rank; i < m; i += 4 * split) {
@@ -295,18 +308,6 @@ gemm_fp4_fewrows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
         }
         __syncwarp();
         cluster_sync_all();  // no CTA leaves while another reads its shared memory
-    }
-
-    // ------------------------------------------------------------- teardown
-    __syncthreads();
-    if (*abort_flag) {
-        if (tid == 0) atomicExch(a.status, INT4L_ERR_DEVICE_TIMEOUT);
-        for (int i = 0; i < 100; ++i) __nanosleep(1000);  // copies in flight land
-        __syncthreads();
-    }
-    if (warp == 1) {
-        tc_fence_after_sync();
-        tmem_dealloc<1>(tmem_base, a.cols);
     }
 }
 

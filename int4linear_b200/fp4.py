@@ -42,8 +42,8 @@ def _check_shape(rows: int, k: int, fmt: str) -> None:
         raise ValueError(f"unknown format {fmt!r}: expected one of {sorted(FORMATS)}")
     if rows < 0 or k <= 0 or k % 32 != 0:
         raise ValueError("need k > 0 and k % 32 == 0")
-    if rows >= 2 ** 31 or k >= 2 ** 31:
-        raise ValueError("rows and k must fit 32 bits")
+    if rows > 2 ** 26 or k > 2 ** 26:
+        raise ValueError("rows and k are at most 2^26")
 
 
 def _check_tensor_scale(ts, fmt: str, device) -> None:

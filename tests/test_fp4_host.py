@@ -26,7 +26,7 @@ def bad_matrices():
     """(matrix, status) pairs that every entry point refuses."""
     return [(matrix(rows=0), 1), (matrix(rows=-1), 1), (matrix(k=0), 1), (matrix(k=48), 2), (matrix(k=16), 2), (matrix(fmt=2), 1), (matrix(fmt=-1), 1),
             (matrix(codes=None), 1), (matrix(scales=None), 1), (matrix(codes=BASE + 8), 3), (matrix(scales=BASE + 4), 3),
-            (matrix(ts=BASE), 1), (matrix(fmt=1, ts=BASE + 2), 3)]
+            (matrix(ts=BASE), 1), (matrix(fmt=1, ts=BASE + 2), 3), (matrix(rows=2 ** 26 + 1), 7), (matrix(k=2 ** 26 + 32), 7)]
 
 
 def test_c_entry_points_refuse_bad_matrices():
@@ -116,7 +116,7 @@ def test_python_refuses_cpu_tensors_and_unknown_names():
         L.Fp4Matrix(torch.zeros((4, 32), dtype=torch.uint8), torch.zeros(512, dtype=torch.uint8), 4, 64)
     with pytest.raises(ValueError):
         fp4._check_shape(4, 64, "fp4")
-    for rows, k in ((4, 48), (4, 0), (-1, 32), (2 ** 31, 32)):
+    for rows, k in ((4, 48), (4, 0), (-1, 32), (2 ** 26 + 1, 32), (1, 2 ** 26 + 32)):
         with pytest.raises(ValueError):
             fp4._check_shape(rows, k, "mxfp4")
     with pytest.raises(ValueError):

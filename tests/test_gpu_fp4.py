@@ -340,6 +340,20 @@ def test_gated_backward(cuda, fmt, act, m, n, k):
     assert none is None and torch.equal(a, dwg) and torch.equal(b, dwu)
 
 
+def test_backward_of_unaligned_gradients(cuda):
+    """Gradients that start on any element, n a multiple of 8 and not."""
+    for m, n in ((40, 136), (40, 133), (700, 264)):
+        x, w = R.matrix(L, m, 96, "mxfp4", 1, cuda), R.matrix(L, n, 96, "mxfp4", 2, cuda)
+        pool = torch.randn((3, m * n + 8), device=cuda).to(torch.bfloat16)
+        for off in (1, 2, 8):
+            a, b, c = (t[off:off + m * n].view(m, n) for t in pool)
+            copies = [t.clone() for t in (a, b, c)]
+            for got, want in zip(L.gated_linear_fp4_backward(a, b, c, x, w, w), L.gated_linear_fp4_backward(*copies, x, w, w)):
+                assert torch.equal(got, want)
+            for got, want in zip(L.linear_fp4_backward(a, x, w), L.linear_fp4_backward(copies[0], x, w)):
+                assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 200, 96), (7, 6000, 64), (130, 400, 320), (60, 1001, 512)])
 def test_gated_backward_of_small_problems_is_as_good_as_one_rounding(cuda, m, n, k):
     """Small problems carry dg and du in two terms: an error of 2^-16 in them, so what is left is the result's rounding."""
@@ -476,6 +490,42 @@ def test_other_streams(cuda):
     torch.cuda.synchronize()
     for y, g in got:
         assert torch.equal(y, want) and all(torch.equal(a, b) for a, b in zip(g, want_g))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_garbage_in_the_row_padding_of_scales(cuda, fmt):
+    """Scale rows beyond the matrix may hold anything, NaN included."""
+    m, n, k = 70, 200, 352
+    nan = 255 if fmt == "mxfp4" else 0x7F
+    mats = [R.matrix(L, r, k, fmt, r, cuda, scale=0.25) for r in (m, n)]
+    dirty = []
+    for q in mats:
+        s = q.scales.clone()
+        t = s.view(-(-q.rows // 128), -1, 32, 4, 4).permute(0, 3, 2, 1, 4)  # [group, row / 32, row % 32, tile, scale]
+        rows = torch.arange(t.shape[0] * 128, device=cuda).view(t.shape[0], 4, 32)
+        t[rows >= q.rows] = nan
+        dirty.append(L.Fp4Matrix(q.codes, s, q.rows, k, fmt, q.tensor_scale))
+    dy, g, u = (torch.randn((m, n), device=cuda).to(torch.bfloat16) for _ in range(3))
+
+    def all_of(x, w):
+        return (L.dequantize_fp4(x), L.linear_fp4(x, w), L.linear_fp4(w, w), L.gated_linear_fp4(x, w, w), *L.linear_fp4_backward(dy, x, w),
+                *L.gated_linear_fp4_backward(dy, g, u, x, w, w))
+
+    for a, b in zip(all_of(*dirty), all_of(*mats)):
+        assert torch.equal(a, b) and torch.isfinite(a).all()
+
+
+def test_infinite_gradients_stay_in_their_rows_and_columns(cuda):
+    m, n, k = 40, 96, 64
+    x, w = R.matrix(L, m, k, "mxfp4", 1, cuda), R.matrix(L, n, k, "mxfp4", 2, cuda)
+    dy = torch.randn((m, n), device=cuda).to(torch.bfloat16)
+    clean = L.linear_fp4_backward(dy, x, w)
+    dy[3, 5] = float("inf")
+    dx, dw = L.linear_fp4_backward(dy, x, w)
+    rows = torch.arange(m, device=cuda) != 3
+    cols = torch.arange(n, device=cuda) != 5
+    assert torch.equal(dx[rows], clean[0][rows]) and torch.equal(dw[cols], clean[1][cols])
+    assert not torch.isfinite(dx[3]).any() and not torch.isfinite(dw[5]).any()
 
 
 def test_repeated_calls_give_the_same_bits(cuda):
