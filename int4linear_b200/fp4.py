@@ -171,9 +171,14 @@ def _run(body, device, stream, inputs):
         return body(handle)
 
 
+_types: dict = {}  # torch type -> INT4L_TYPE_*, filled by the first call
+
+
 def _type_of(dtype) -> int:
-    import torch
-    t = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}.get(dtype)
+    if not _types:
+        import torch
+        _types.update({torch.bfloat16: 0, torch.float16: 1, torch.float32: 2})
+    t = _types.get(dtype)
     if t is None:
         raise TypeError(f"expected bfloat16, float16 or float32, not {dtype}")
     return t

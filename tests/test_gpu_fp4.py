@@ -515,6 +515,39 @@ def test_garbage_in_the_row_padding_of_scales(cuda, fmt):
         assert torch.equal(a, b) and torch.isfinite(a).all()
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_offsets_beyond_32_bits(cuda, fmt):
+    """More than 2^32 elements in x (quantisation, expansion) and in y and dy (products): the last rows are right."""
+    rows, cols = 140000, 32768
+    big = torch.zeros((rows, cols), dtype=torch.bfloat16, device=cuda)
+    big[-300:] = torch.randn((300, cols), device=cuda).to(torch.bfloat16)
+    q = L.quantize_fp4(big, fmt)
+    tail = L.quantize_fp4(big[-300:], fmt)
+    assert torch.equal(q.codes[-300:], tail.codes) and not q.codes[:-300].any()
+    L.dequantize_fp4(q, out=big)
+    assert torch.equal(big[-300:], L.dequantize_fp4(tail, dtype=torch.bfloat16))
+    del q
+    k = 64
+    x, w = R.matrix(L, rows, k, fmt, 1, cuda), R.matrix(L, cols, k, fmt, 2, cuda)
+    xv = R.values(L.Fp4Matrix.from_rows(x.codes[-300:], x.scale_rows()[-300:], fmt, x.tensor_scale))
+    wv = R.values(w)
+    L.linear_fp4(x, w, out=big)
+    want = xv @ wv.t()
+    close(big[-300:], want, want.abs() * 2.0 ** -8 + R.product_bound(xv, wv) * 1.01)
+    L.gated_linear_fp4(x, w, w, out=big)
+    want = R.act(want, "silu") * want
+    assert (big[-300:].double() - want).norm() <= 2.0 ** -8 * want.norm()
+    big.zero_()
+    big[-300:] = torch.randn((300, cols), device=cuda).to(torch.bfloat16)
+    dx, dw = L.linear_fp4_backward(big, x, w)
+    d = big[-300:].double()
+    for got, a, b in ((dx[-300:], d, wv), (dw, d.t(), xv)):
+        want, s = a @ b, a.abs() @ b.abs()
+        # the rows before are zeros: the sums take as many steps, of which only the last add anything
+        close(got, want, want.abs() * 2.0 ** -8 + (a.shape[1] / 16 + 2) * 2.0 ** -23 * s * 1.01)
+    assert not dx[:-300].any()
+
+
 def test_infinite_gradients_stay_in_their_rows_and_columns(cuda):
     m, n, k = 40, 96, 64
     x, w = R.matrix(L, m, k, "mxfp4", 1, cuda), R.matrix(L, n, k, "mxfp4", 2, cuda)
