@@ -38,7 +38,7 @@ __device__ __forceinline__ size_t fp4_scale_word(int row, int kt, int ktiles)
 }
 #endif
 
-enum GateAct { kActNone = -1, kActSilu = 0, kActGelu = 1, kActGeluTanh = 2 };
+enum GateAct { kActSilu = INT4L_ACT_SILU, kActGelu = INT4L_ACT_GELU, kActGeluTanh = INT4L_ACT_GELU_TANH };
 
 // One product: y = x w^T (w_up null), or h = act(x w^T) * (x w_up^T).
 struct Fp4Problem {

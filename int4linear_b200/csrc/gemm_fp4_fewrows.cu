@@ -16,6 +16,9 @@
 //     warp 0      TMA (as in gemm_fp4.cu)
 //     warp 1      tcgen05.cp of the scales and UMMAs
 //     all 4       epilogue
+//
+// Measured, per launch in a graph with weights from HBM: 1 x 14336 x 4096 mxfp4 8.8 us (3.5 TB/s), 16 rows nvfp4 9.7, gated
+// 16 rows mxfp4 15.1 (4.1 TB/s), 1 x 4096 x 4096 6.1, 16 x 28672 x 8192 24 (5.2 TB/s); the fixed part is 4 us.
 #include "epilogue.cuh"
 #include "fp4.cuh"
 #include "gate.cuh"
