@@ -612,13 +612,13 @@ Plan plan(long long m, long long n, long long k, bool gated, bool want_dx, bool 
     // What is decided here does not depend on which gradients are wanted, so their bits do not either.
     const double tiles_dx = static_cast<double>(p.dx.tiles_m) * tn, tiles_dw = static_cast<double>(matrices) * p.dw.tiles_m * tn;
     const double load = (tiles_dx * matrices * steps_n + tiles_dw * steps_m) / kPlanWorkers;  // steps of a worker
-    // Two terms for dg and du where twice the steps are a few microseconds, or where there are so few values of them
-    // that the time goes into the weights.
     // Expanded operands go to memory and come back: four times their bytes, twice, which few tokens do not repay, and
     // it is a launch of its own.  The in-kernel expansion holds the products below 1.4 PFLOP/s.  Measured, in-kernel
     // against expanded: mxfp4 64 x 8192 x 4096 49 us and 66, 256 rows 60 and 69, 512 rows 78 and 85, gated 512 rows 152
     // and 158, 128 x 1024 x 1024 16 and 24; nvfp4 1024 rows 109 and 111; 4096 x 4096 x 8192 403 and 351.
     p.unpack = m <= 512 || load <= 24.0;
+    // Two terms for dg and du where twice the steps are a few microseconds, or where there are so few values of them
+    // that the time goes into the weights.
     p.fine = gated && (2.0 * load <= 24.0 || m * n <= 65536);
     if (p.fine) {
         p.dx.segments *= 2;
