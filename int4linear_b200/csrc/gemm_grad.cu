@@ -37,6 +37,8 @@
 //
 // Measured: 4096 x 4096 x 8192 nvfp4 360 us (1.53 PFLOP/s, tensor pipe 91 % busy at the 1.5 GHz the power limit leaves), gated
 // 4096 x 14336 x 4096 mxfp4 1.36 ms, of which the preparation takes 0.14 (it writes 0.7 GB).
+#include <cmath>
+
 #include "epilogue.cuh"
 #include "fp4_expand.cuh"
 #include "gate.cuh"
@@ -599,6 +601,7 @@ struct Plan {
 constexpr int kPlanWorkers = 74;  // CTA pairs of a B200
 constexpr int kTileSteps = 6;     // a tile's epilogue, in steps: it runs beside the next tile's steps, and is longer than few of them
 constexpr int kMinPart = 8;       // steps of a part: less would be the time of a tile's start and end
+constexpr int kMaxParts = 74;
 constexpr int kMinSaving = 24;    // steps (0.28 us each) that pay for the partial sums' way and the third launch
 
 Plan plan(long long m, long long n, long long k, bool gated, bool want_dx, bool want_dw)
@@ -625,11 +628,14 @@ Plan plan(long long m, long long n, long long k, bool gated, bool want_dx, bool 
         p.dw.segments *= 2;
     }
     auto cut = [&](Kind& kind, double tiles) {
-        // (no more parts than workers: one item too many would double the time)
+        // The time of the busiest worker, in steps, if only this kind existed; a part costs about kTileSteps besides.
         const int steps = kind.segments * kind.seg_steps;
-        int parts = tiles < kPlanWorkers ? static_cast<int>(kPlanWorkers / tiles) : 1;
-        if (parts > steps / kMinPart) parts = steps / kMinPart;
-        if (parts > 1 && steps - steps / parts >= kMinSaving) kind.parts = parts;
+        if (tiles >= 4.0 * kPlanWorkers) return;
+        double best = std::ceil(tiles / kPlanWorkers) * (steps + kTileSteps) - kMinSaving;
+        for (int parts = 2; parts <= kMaxParts && steps / parts >= kMinPart; ++parts) {
+            const double time = std::ceil(tiles * parts / kPlanWorkers) * ((steps + parts - 1) / parts + kTileSteps);
+            if (time < best) { best = time; kind.parts = parts; }
+        }
     };
     cut(p.dx, tiles_dx);
     cut(p.dw, tiles_dw);
