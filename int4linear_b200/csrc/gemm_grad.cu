@@ -498,37 +498,53 @@ grad_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Grad
             tc_fence_after_sync();
             const int row0 = (t.tm * 2 + static_cast<int>(cta_rank)) * kBM + sp * 32;
             const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(sp * 32) << 16) + buf * kBN;
+            const int col_first = t.tn * kBN;
+            const int chunks = row0 < t.kind->rows ? min(kBN, t.kind->cols - col_first + 63) / 64 : 0;  // of 64 columns
+            if (!whole) {
 #pragma unroll 1
-            for (int c = 0; c < kBN; c += 64) {
-                const int col0 = t.tn * kBN + c;
-                if (row0 >= t.kind->rows || col0 >= t.kind->cols) break;
-                uint32_t v[64], h[32];
-                load64(t_addr + c, v);
-                tmem_ld_wait();
-                if (!whole) {
-                    if (row0 + lane < t.kind->rows) {
-                        float* dst = partial + static_cast<size_t>(row0 + lane) * t.kind->cols + col0;
+                for (int c = 0; c < chunks; ++c) {
+                    uint32_t v[64];
+                    load64(t_addr + 64 * c, v);
+                    tmem_ld_wait();
+                    const int col0 = col_first + 64 * c;
+                    if (row0 + lane >= t.kind->rows) continue;
+                    float* dst = partial + static_cast<size_t>(row0 + lane) * t.kind->cols + col0;
 #pragma unroll
-                        for (int q = 0; q < 16; ++q)  // (cols is a multiple of 32)
-                            if (col0 + 4 * q < t.kind->cols) reinterpret_cast<uint4*>(dst)[q] = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+                    for (int q = 0; q < 16; ++q)  // (cols is a multiple of 32)
+                        if (col0 + 4 * q < t.kind->cols) reinterpret_cast<uint4*>(dst)[q] = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+                }
+            } else if (chunks > 0) {
+                // 32 columns at a time, the next 32 on their way from tensor memory meanwhile.
+                uint32_t v0[32], v1[32];
+                auto put32 = [&](const uint32_t (&v)[32], uint32_t stg, int half) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t h[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) h[e] = pack16<false>(__uint_as_float(v[8 * q + 2 * e]) * alpha, __uint_as_float(v[8 * q + 2 * e + 1]) * alpha);
+                        sts128(stg + lane * 128 + (((4 * half + q) ^ (lane & 7)) << 4), make_uint4(h[0], h[1], h[2], h[3]));
                     }
-                    continue;
+                };
+                tmem_ld_32x32(t_addr, v0);
+#pragma unroll 1
+                for (int c = 0; c < chunks; ++c) {
+                    const uint32_t stg = stage0 + (chunk_no & 1u) * kStoreStage;
+                    if (lane == 0) tma_store_wait_read<1>();
+                    __syncwarp();
+                    tmem_ld_wait();
+                    tmem_ld_32x32(t_addr + 64 * c + 32, v1);
+                    put32(v0, stg, 0);
+                    tmem_ld_wait();
+                    if (c + 1 < chunks) tmem_ld_32x32(t_addr + 64 * c + 64, v0);
+                    put32(v1, stg, 1);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_2d(out, stg, col_first + 64 * c, row0);
+                        tma_store_commit();
+                    }
+                    ++chunk_no;
                 }
-#pragma unroll
-                for (int j = 0; j < 32; ++j) h[j] = pack16<false>(__uint_as_float(v[2 * j]) * alpha, __uint_as_float(v[2 * j + 1]) * alpha);
-                const uint32_t stg = stage0 + (chunk_no & 1u) * kStoreStage;
-                if (lane == 0) tma_store_wait_read<1>();
-                __syncwarp();
-#pragma unroll
-                for (int q = 0; q < 8; ++q)
-                    sts128(stg + lane * 128 + ((q ^ (lane & 7)) << 4), make_uint4(h[4 * q], h[4 * q + 1], h[4 * q + 2], h[4 * q + 3]));
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                    tma_store_2d(out, stg, col0, row0);
-                    tma_store_commit();
-                }
-                ++chunk_no;
             }
             tc_fence_before_sync();
             __syncwarp();
