@@ -15,19 +15,31 @@ constexpr float kGeluA = 0.044715f;
 // Two ulp of exp and of the reciprocal: the result is rounded to 16 bits.  (exp overflows to infinity for
 // v < -88, whose reciprocal is the 0 that is wanted.)
 __device__ __forceinline__ float logistic(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
-// The normal distribution function and exp(-v^2 / 2), by the rational form 7.1.26 of Abramowitz and Stegun,
-// "Handbook of Mathematical Functions": erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + p x), absolute error
-// at most 1.5e-7, which is that of 1 + erf in fp32; the tail is not the difference of two near values.  (With erfcf
-// the epilogue, not the products, set the time of a gated call: 302 against 183 us at 4096 x 14336 x 4096.)
+// 1 / v for v >= 1, to one unit in the last place; 0 from 2^126 on.
+__device__ __forceinline__ float reciprocal(float v)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+// The normal distribution function and exp(-v^2 / 2).  The lower tail is the density times t P(t), t = 1 / (1 + 0.362 |v|),
+// P the polynomial of degree 6 for which the largest RELATIVE error against erfc(|v| / sqrt 2) / 2 is least over [0, 14.6]
+// (weighted least squares, the weights multiplied by the error until it levels out: Lawson, "Contributions to the theory of
+// linear least maximum approximation", 1961): 0.9e-6, 1.2e-6 evaluated in fp32, a four-hundredth of half a step of fp16.  So
+// g P(g) keeps its bits as far out as the density does.  (With erfcf the epilogue, not the products, set the time of a
+// gated call: 302 us at 4096 x 14336 x 4096.)
 __device__ __forceinline__ float normal_cdf(float v, float& density)
 {
-    density = __expf(-0.5f * v * v);
-    const float t = __fdividef(1.0f, 1.0f + 0.3275911f * 0.7071067811865476f * fabsf(v));
-    float q = fmaf(t, 1.061405429f, -1.453152027f);
-    q = fmaf(t, q, 1.421413741f);
-    q = fmaf(t, q, -0.284496736f);
-    q = fmaf(t, q, 0.254829592f);
-    q *= 0.5f * t * density;
+    const float z = v * 0.84932180f;  // sqrt(log2(e) / 2)
+    density = exp2f(-z * z);
+    const float t = reciprocal(fmaf(0.362f, fabsf(v), 1.0f));
+    float q = fmaf(t, 0.0476089977f, -0.178899616f);
+    q = fmaf(t, q, 0.175130531f);
+    q = fmaf(t, q, 0.029837992f);
+    q = fmaf(t, q, 0.139068753f);
+    q = fmaf(t, q, 0.142753929f);
+    q = fmaf(t, q, 0.144499421f);
+    q *= t * density;
     return v < 0.0f ? q : 1.0f - q;
 }
 
