@@ -67,7 +67,7 @@ def slope(g, act):
 
 
 @pytest.mark.parametrize("m", [32, 96])
-@pytest.mark.parametrize("act,top", [("silu", 1.0), ("gelu", 1.0), ("gelu", 2.0), ("gelu_tanh", 1.0)])
+@pytest.mark.parametrize("act,top", [("silu", 1.0), ("silu", 16.0), ("gelu", 1.0), ("gelu", 2.0), ("gelu_tanh", 1.0)])
 def test_activation_is_within_one_rounding_everywhere(cuda, m, act, top):
     """g = each value of w_gate (x is the identity, up is 1), down to where act(g) leaves the output type."""
     n, k = 1000, 96
@@ -85,11 +85,13 @@ def test_activation_is_within_one_rounding_everywhere(cuda, m, act, top):
         err = (h.double() - want).abs()
         # (results and intermediates below 2^-126 have fewer bits)
         bound = want.abs() * (half + relative(g, act) * (1 + half)) + TINY[dtype] + (1 + g.abs()) * 2.0 ** -146
+        if act != "gelu":  # 1 / (1 + exp(-v)) is 0 where the divisor passes 2^126: the factor of g is below 2^-126 there
+            bound += torch.where(exponent(g, act) > 126 * math.log(2), g.abs() * 2.0 ** -126, torch.zeros_like(g))
         worst = ((err - bound) / want.abs().clamp(min=2.0 ** -140)).max().item()
         assert (err <= bound).all(), worst
 
 
-@pytest.mark.parametrize("act", ["gelu"])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
 def test_gate_gradients_far_out(cuda, act):
     """dg and du come through identity weights: dx = dg with w_gate = 1, w_up = 0, and dx = du the other way round."""
     n = 128
