@@ -81,7 +81,9 @@ __device__ __forceinline__ void gate_act_slope(float g, float& act, float& slope
         float c;
         const float s = logistic(z2, c);
         act = g * s;
-        slope = s * (1.0f + g * c * 2.0f * kGeluC * (1.0f + 3.0f * kGeluA * g * g));
+        // Beyond +-32 the slope is 0 or 1 (so are s and c); the factor between them must not overflow there.
+        const float near = fminf(fmaxf(g, -32.0f), 32.0f);
+        slope = s * (1.0f + near * c * 2.0f * kGeluC * (1.0f + 3.0f * kGeluA * near * near));
     }
 }
 

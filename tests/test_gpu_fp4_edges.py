@@ -91,7 +91,7 @@ def test_activation_is_within_one_rounding_everywhere(cuda, m, act, top):
         assert (err <= bound).all(), worst
 
 
-@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
 def test_gate_gradients_far_out(cuda, act):
     """dg and du come through identity weights: dx = dg with w_gate = 1, w_up = 0, and dx = du the other way round."""
     n = 128
@@ -114,3 +114,16 @@ def test_gate_gradients_far_out(cuda, act):
     want = torch.where(gd < -1e3, torch.zeros_like(gd), torch.where(gd > 1e3, gd, value(gd.clamp(-1e3, 1e3), act)))
     err = (du.double() - want).abs()
     assert torch.isfinite(du).all() and (err <= want.abs() * (2.0 ** -8 + (rel + 2.0 ** -16) * 1.01) + small + tail).all(), err.max()
+
+
+def test_nan_gate_stays_nan(cuda):
+    for act in ("silu", "gelu", "gelu_tanh"):
+        n = 64
+        g = torch.zeros((2, n), dtype=torch.bfloat16, device=cuda)
+        g[1, 5] = float("nan")
+        one = torch.ones_like(g)
+        x, w = eye(2, n, "mxfp4", cuda), eye(n, n, "mxfp4", cuda)
+        dx, dwg, dwu = L.gated_linear_fp4_backward(one, g, one, x, w, w, act)
+        assert torch.isnan(dx[1]).all() and torch.isfinite(dx[0]).all()
+        for d in (dwg, dwu):
+            assert torch.isnan(d[5]).all() and torch.isfinite(d[:5]).all() and torch.isfinite(d[6:]).all()
