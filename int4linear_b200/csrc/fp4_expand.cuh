@@ -22,6 +22,18 @@ __device__ __forceinline__ float from_e4m3(uint32_t byte)
     return __half2float(__ushort_as_half(static_cast<unsigned short>(h2 & 0xFFFFu)));
 }
 
+// a b in fp32.  kOdd: rounded to odd (cut off, the last bit set where something was cut), so that rounding the result to 16 bits
+// rounds the product once: a product beside a tie does not land on it.  (A remainder below 2^-150 is lost, which takes a
+// product below 2^-119.)  Three more instructions per value: 8192 x 8192 nvfp4 to bf16 28.7 -> 32.8 us.
+template <bool kOdd>
+__device__ __forceinline__ float times(float a, float b)
+{
+    if constexpr (!kOdd) return a * b;
+    const float p = __fmul_rz(a, b);
+    // (a NaN remainder comes with an infinite or NaN product, which stays as it is)
+    return fabsf(fmaf(a, b, -p)) > 0.0f ? __uint_as_float(__float_as_uint(p) | 1u) : p;
+}
+
 // A warp's unit: 32 kE consecutive elements (kE per lane) of four consecutive rows.  Both kernels were first bound by
 // instructions, most of them addresses: with a row of its own per step they took 143 (mxfp4), 236 (nvfp4) and 116
 // (expansion) instructions for eight elements; a unit's rows share the address arithmetic.
@@ -89,7 +101,7 @@ __device__ __forceinline__ void fp4_expand_block(uint32_t block_index, const uin
         for (int b = 0; b < 4; ++b) {
             const float2 c = __half22float2(*reinterpret_cast<const __half2*>(&h2[b]));
             float lo = c.x * s, hi = c.y * s;  // exact
-            if (scaled) { lo *= ts; hi *= ts; }
+            if (scaled) { lo = times<kType != INT4L_TYPE_F32>(lo, ts); hi = times<kType != INT4L_TYPE_F32>(hi, ts); }
             if constexpr (kType == INT4L_TYPE_BF16) reinterpret_cast<uint32_t*>(out)[b] = pack16<false>(lo, hi);
             else if constexpr (kType == INT4L_TYPE_F16) reinterpret_cast<uint32_t*>(out)[b] = pack16<true>(lo, hi);
             else { out[2 * b] = lo; out[2 * b + 1] = hi; }

@@ -127,3 +127,50 @@ def test_nan_gate_stays_nan(cuda):
         assert torch.isnan(dx[1]).all() and torch.isfinite(dx[0]).all()
         for d in (dwg, dwu):
             assert torch.isnan(d[5]).all() and torch.isfinite(d[:5]).all() and torch.isfinite(d[6:]).all()
+
+
+@pytest.mark.parametrize("dtype,bits", [(torch.bfloat16, 8), (torch.float16, 11)])
+def test_dequantize_rounds_once(cuda, dtype, bits):
+    """Tensor scales for which code x scale x tensor scale lies beside a tie of the 16-bit type, nearer to it than half a step of
+    fp32: a product that is rounded to fp32 first lands on the tie and then goes to the even side, right or wrong."""
+    mant = {c * (1 + s / 8) for c in (1.0, 1.5) for s in range(8)}
+    gen = torch.Generator().manual_seed(bits)
+    picks = []
+    for _ in range(400):
+        p = (1 + torch.randint(0, 2 ** (bits - 1), (1,), generator=gen).item() * 2.0 ** (1 - bits) + 2.0 ** -bits)  # a tie in [1, 2)
+        a = sorted(mant)[torch.randint(0, len(mant), (1,), generator=gen).item()]
+        ts = torch.tensor([p / a], dtype=torch.float64).float()
+        exact = ts.double().item() * a  # 6 bits times 24: exact in 64
+        rounded = torch.tensor(exact, dtype=torch.float64).float().double().item()
+        if rounded == p and exact != p:
+            lo, hi = p - 2.0 ** -bits, p + 2.0 ** -bits
+            picks.append((a, ts, lo if exact < p else hi))
+    assert len(picks) >= 20
+    wrong = 0
+    for a, ts, want in picks:
+        mags = [(c, s) for c in range(1, 8) for s in range(0x38, 0x40) if R.MAG[c] * R.e4m3_values()[s].item() == a]
+        c, s = mags[0]
+        q = L.Fp4Matrix.from_rows(torch.full((1, 16), c | (c << 4) | 0x80, dtype=torch.uint8, device=cuda),
+                                  torch.full((1, 2), s, dtype=torch.uint8, device=cuda), "nvfp4", ts.to(cuda))
+        got = L.dequantize_fp4(q, dtype=dtype).double().view(-1)
+        wrong += int((got[0::2] != want).any()) + int((got[1::2] != -want).any())
+    assert wrong == 0, f"{wrong} of {2 * len(picks)} values rounded twice"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("ts", [0.0, math.inf, -math.inf, math.nan, 3.0e38, -0.37, 1e-38, 2.0 ** -140])
+def test_dequantize_under_extreme_tensor_scales(cuda, dtype, ts):
+    q = R.matrix(L, 40, 96, "nvfp4", 4, cuda)
+    sb = q.scale_rows()
+    sb[3, 2] = 0x7F
+    q = L.Fp4Matrix.from_rows(q.codes, sb, "nvfp4", torch.tensor([ts], device=cuda))
+    want = R.values(q)
+    got = L.dequantize_fp4(q, dtype=dtype).double()
+    # What rounds beyond the largest value is infinite; products of 64-bit values never overflow before.
+    top = (2 - 2.0 ** (-7 if dtype == torch.bfloat16 else -10)) * 2.0 ** (127 if dtype == torch.bfloat16 else 15)
+    half_step = top * HALF[dtype] / 2
+    want = torch.where(want.abs() >= top + half_step, torch.copysign(torch.full_like(want, math.inf), want), want)
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.isinf(got), torch.isinf(want))
+    fine = torch.isfinite(want)
+    assert torch.equal(torch.signbit(got[torch.isinf(want)]), torch.signbit(want[torch.isinf(want)]))
+    assert ((got - want).abs()[fine] <= want.abs()[fine] * HALF[dtype] + TINY[dtype]).all()
