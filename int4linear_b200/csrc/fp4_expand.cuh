@@ -22,6 +22,28 @@ __device__ __forceinline__ float from_e4m3(uint32_t byte)
     return __half2float(__ushort_as_half(static_cast<unsigned short>(h2 & 0xFFFFu)));
 }
 
+// The value of a scale byte, NaN included.
+template <bool kBlock16>
+__device__ __forceinline__ float fp4_scale(uint32_t byte)
+{
+    if constexpr (kBlock16) return from_e4m3(byte);  // 0x7F converts to NaN
+    // 2^(b - 127); 2^-127 is subnormal
+    return byte == 0xFFu ? __uint_as_float(0x7FFFFFFFu) : __uint_as_float(byte ? byte << 23 : 0x00400000u);
+}
+
+// Eight codes -> eight halves.
+__device__ __forceinline__ void fp4_codes_to_halves(uint32_t word, uint32_t (&h2)[4])
+{
+    asm("{\n\t"
+        ".reg .b8 c0, c1, c2, c3;\n\t"
+        "mov.b32 {c0, c1, c2, c3}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, c0;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %1, c1;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, c2;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %3, c3;\n\t"
+        "}\n" : "=r"(h2[0]), "=r"(h2[1]), "=r"(h2[2]), "=r"(h2[3]) : "r"(word));
+}
+
 // a b in fp32.  kOdd: rounded to odd (cut off, the last bit set where something was cut), so that rounding the result to 16 bits
 // rounds the product once: a product beside a tie does not land on it.  (A remainder below 2^-150 is lost, which takes a
 // product below 2^-119.)  Three more instructions per value: 8192 x 8192 nvfp4 to bf16 28.7 -> 32.8 us.
@@ -79,23 +101,10 @@ __device__ __forceinline__ void fp4_expand_block(uint32_t block_index, const uin
 #pragma unroll
     for (int i = 0; i < kUnitRows; ++i, d += k) {
         if (u.row0 + i >= rows) break;
-        float s;
-        if constexpr (kBlock16) {
-            s = from_e4m3(byte[i]);  // 0x7F converts to NaN
-        } else {
-            // 2^(b - 127); 2^-127 is subnormal
-            s = byte[i] == 0xFFu ? __uint_as_float(0x7FFFFFFFu) : __uint_as_float(byte[i] ? byte[i] << 23 : 0x00400000u);
-        }
+        const float s = fp4_scale<kBlock16>(byte[i]);
         const bool scaled = kBlock16 && ts != 1.0f;
-        uint32_t h2[4];  // the codes as eight halves
-        asm("{\n\t"
-            ".reg .b8 c0, c1, c2, c3;\n\t"
-            "mov.b32 {c0, c1, c2, c3}, %4;\n\t"
-            "cvt.rn.f16x2.e2m1x2 %0, c0;\n\t"
-            "cvt.rn.f16x2.e2m1x2 %1, c1;\n\t"
-            "cvt.rn.f16x2.e2m1x2 %2, c2;\n\t"
-            "cvt.rn.f16x2.e2m1x2 %3, c3;\n\t"
-            "}\n" : "=r"(h2[0]), "=r"(h2[1]), "=r"(h2[2]), "=r"(h2[3]) : "r"(word[i]));
+        uint32_t h2[4];
+        fp4_codes_to_halves(word[i], h2);
         __align__(16) T out[8];
 #pragma unroll
         for (int b = 0; b < 4; ++b) {

@@ -231,27 +231,20 @@ __device__ __forceinline__ void mbar_arrive_after_warp(uint32_t bar, uint32_t lo
 }
 
 // 64 codes of one row and their scales (a word of 4 in nvfp4, 2 bytes in mxfp4) -> 64 bf16, eight 16-byte chunks of a
-// 128-byte-swizzled row.
+// 128-byte-swizzled row.  Rows outside the matrix are 0 whatever their scale; factor is 0 under a tensor scale of 0, else 1 (a
+// NaN scale stays NaN).
 template <bool kBlock16>
-__device__ __forceinline__ void expand_row(uint4 lo, uint4 hi, uint32_t scale_word, bool zero, uint32_t row_at, int row)
+__device__ __forceinline__ void expand_row(uint4 lo, uint4 hi, uint32_t scale_word, bool outside, float factor, uint32_t row_at, int row)
 {
     const uint32_t words[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
         const uint32_t byte = (scale_word >> (8 * (kBlock16 ? c / 2 : c / 4))) & 0xFFu;
-        float sc;
-        if constexpr (kBlock16) sc = from_e4m3(byte);
-        else sc = byte == 0xFFu ? __uint_as_float(0x7FFFFFFFu) : __uint_as_float(byte ? byte << 23 : 0x00400000u);
-        if (zero) sc = 0.0f;
+        float sc = fp4_scale<kBlock16>(byte);
+        if (kBlock16) sc *= factor;
+        if (outside) sc = 0.0f;
         uint32_t h2[4];
-        asm("{\n\t"
-            ".reg .b8 c0, c1, c2, c3;\n\t"
-            "mov.b32 {c0, c1, c2, c3}, %4;\n\t"
-            "cvt.rn.f16x2.e2m1x2 %0, c0;\n\t"
-            "cvt.rn.f16x2.e2m1x2 %1, c1;\n\t"
-            "cvt.rn.f16x2.e2m1x2 %2, c2;\n\t"
-            "cvt.rn.f16x2.e2m1x2 %3, c3;\n\t"
-            "}\n" : "=r"(h2[0]), "=r"(h2[1]), "=r"(h2[2]), "=r"(h2[3]) : "r"(words[c]));
+        fp4_codes_to_halves(words[c], h2);
         uint32_t out[4];
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
@@ -473,9 +466,9 @@ grad_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Grad
                 if (!kBlock16) word >>= 16 * h;
                 mbar_arrive_after_warp(pk_empty(ps), lo.x ^ lo.y ^ lo.z ^ lo.w ^ hi.x ^ hi.y ^ hi.z ^ hi.w ^ word, lane);
                 // Rows beyond the matrix have code 0 (read out of bounds) and no defined scale.
-                const bool zero = k0 + row >= (t.weight ? a.m : a.n) || ts[which] == 0.0f;
+                const bool outside = k0 + row >= (t.weight ? a.m : a.n);
                 if (!mbar_wait_warp(empty(s), (r & 1u) ^ 1u, abort_flag)) { alive = false; break; }
-                expand_row<kBlock16>(lo, hi, word, zero, ring + s * kStage + (2 + h) * kChunk + row * 128, row);
+                expand_row<kBlock16>(lo, hi, word, outside, ts[which] == 0.0f ? 0.0f : 1.0f, ring + s * kStage + (2 + h) * kChunk + row * 128, row);
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster(full(s), 0);

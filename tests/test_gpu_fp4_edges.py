@@ -174,3 +174,29 @@ def test_dequantize_under_extreme_tensor_scales(cuda, dtype, ts):
     fine = torch.isfinite(want)
     assert torch.equal(torch.signbit(got[torch.isinf(want)]), torch.signbit(want[torch.isinf(want)]))
     assert ((got - want).abs()[fine] <= want.abs()[fine] * HALF[dtype] + TINY[dtype]).all()
+
+
+# The second takes the form in which the operands are expanded by a launch of their own.
+@pytest.mark.parametrize("m,n,k", [(70, 200, 96), (1030, 4100, 1056)])
+def test_nan_block_under_a_tensor_scale_of_zero(cuda, m, n, k):
+    """NaN times 0 is NaN in the products and in the expansion, so it is in the gradients."""
+    def with_nan(rows, seed, row, block):
+        q = R.matrix(L, rows, k, "nvfp4", seed, cuda)
+        sb = q.scale_rows()
+        sb[row, block] = 0x7F
+        return L.Fp4Matrix.from_rows(q.codes, sb, "nvfp4", torch.zeros(1, device=cuda))
+
+    x, w = with_nan(m, 1, m - 1, 2), with_nan(n, 2, n - 1, 4)
+    dy = torch.randn((m, n), device=cuda).to(torch.bfloat16)
+    dx, dw = L.linear_fp4_backward(dy, x, w)
+    y = L.linear_fp4(x, w)
+    assert torch.isnan(y[m - 1]).all() and torch.isnan(y[:, n - 1]).all() and not y[:m - 1, :n - 1].any()
+    for d, at in ((dx, 4), (dw, 2)):
+        hit = torch.zeros(k, dtype=torch.bool, device=cuda)
+        hit[16 * at:16 * at + 16] = True
+        assert torch.isnan(d[:, hit]).all() and not d[:, ~hit].any()
+    gdx, dwg, dwu = L.gated_linear_fp4_backward(dy, dy, dy, x, w, w)
+    for d, at in ((gdx, 4), (dwg, 2), (dwu, 2)):
+        hit = torch.zeros(k, dtype=torch.bool, device=cuda)
+        hit[16 * at:16 * at + 16] = True
+        assert torch.isnan(d[:, hit]).all() and not d[:, ~hit].any()
