@@ -198,8 +198,17 @@ def _check_out(out, shape, dtype, device, name="out"):
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {list(shape)} on the operands' device")
 
 
-def quantize_fp4(x, format: str = "mxfp4", tensor_scale=None, out: Fp4Matrix | None = None, stream=None) -> Fp4Matrix:
+def _wanted_format(format: str | None, out: Fp4Matrix | None) -> str:
+    if out is None:
+        return "mxfp4" if format is None else format
+    if format is not None and format != out.format:
+        raise ValueError(f"out is {out.format}, not {format}")
+    return out.format
+
+
+def quantize_fp4(x, format: str | None = None, tensor_scale=None, out: Fp4Matrix | None = None, stream=None) -> Fp4Matrix:
     """Quantise a CUDA matrix [rows, k] of bfloat16, float16 or float32 (k % 32 == 0; rows may be strided).
+    `format`: "mxfp4" or "nvfp4"; None is that of `out`, or "mxfp4".
 
     mxfp4: scale 2^(floor(log2 amax) - 2) per 32 elements.  nvfp4: the values are multiplied by 1 / tensor_scale,
     scale = amax / 6 rounded to e4m3 per 16 elements.  Codes are rounded to nearest, ties to even, and saturate
@@ -210,6 +219,7 @@ def quantize_fp4(x, format: str = "mxfp4", tensor_scale=None, out: Fp4Matrix | N
     rows, k = x.shape
     device = x.device
     t = _type_of(x.dtype)
+    format = _wanted_format(format, out)
     if out is not None:
         if out.shape != (rows, k) or out.device != device or tensor_scale is not None:
             raise ValueError("out must have the shape and device of x, and brings its own tensor_scale")
