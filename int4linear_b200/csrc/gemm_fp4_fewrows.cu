@@ -21,6 +21,7 @@
 // 16 rows mxfp4 15.1 (4.1 TB/s), 1 x 4096 x 4096 6.1, 16 x 28672 x 8192 24 (5.2 TB/s); the fixed part is 4 us.
 #include "epilogue.cuh"
 #include "fp4.cuh"
+#include "fp4_fewrows_plan.cuh"
 #include "gate.cuh"
 #include "ptx.cuh"
 
@@ -28,26 +29,14 @@ namespace i4l {
 
 namespace {
 
-constexpr int kRows = 128;        // rows of w per tile
-constexpr int kStepBytes = 128, kStepK = 256;
+constexpr int kRows = kFewRowsTile;
+constexpr int kStepBytes = kFewRowsStepBytes, kStepK = kFewRowsStepK;
 constexpr int kThreads = 128;
-constexpr int kMaxStages = 3;
-constexpr int kSmShared = 228 * 1024;  // of an SM; each CTA takes 1 KB more than it asks for
-constexpr int kSharedPerCol = 448;     // least shared memory per tensor-memory column
-static_assert(kSmShared / kSharedPerCol < 512 + 128, "no mixture of CTAs may exceed the 512 columns");
+constexpr int kMaxStages = kFewRowsMaxStages;
 
 template <bool kBlock16, bool kGated>
-struct Geo {
-    static constexpr int kTilesK = kBlock16 ? 4 : 2;
-    static constexpr int kW = kGated ? 2 : 1;                 // weight matrices
-    static constexpr int kScaleBytes = kTilesK * kScaleTileBytes;
-    static constexpr int kScaleCols = 4 * kTilesK * (kW + 1);  // tensor-memory columns of a stage's scales
-    static constexpr int kCodesW = kRows * kStepBytes;
-    // Layout of a stage: w codes, scales (w, x), then the x codes (rounded up: a stage starts on 1024 bytes).
-    static constexpr int kOffScales = kW * kCodesW;
-    static constexpr int kOffX = kOffScales + (kW + 1) * kScaleBytes;
-    static_assert(kOffX % 1024 == 0, "x tile must keep the swizzle alignment");
-};
+using Geo = FewRowsGeo<kBlock16, kGated>;
+static_assert(Geo<false, false>::kScaleBytes == 2 * kScaleTileBytes, "scale tile");
 
 struct Args {
     const float* ts_x; const float* ts_w; const float* ts_w_up;
@@ -324,7 +313,7 @@ int scale_map(DeviceCtx* ctx, CUtensorMap* out, const Fp4& q)
 template <bool kBlock16, bool kGated>
 int launch_cfg(DeviceCtx* ctx, const Fp4Problem& p, cudaStream_t stream)
 {
-    using G = Geo<kBlock16, kGated>;
+    const FewRowsPlan l = fewrows_plan<kBlock16, kGated>(p.m, p.n, p.k, ctx->sm_count);
     Args a = {};
     a.ts_x = p.x.tensor_scale; a.ts_w = p.w.tensor_scale; a.ts_w_up = p.w_up.tensor_scale;
     a.bias = p.bias;
@@ -332,42 +321,13 @@ int launch_cfg(DeviceCtx* ctx, const Fp4Problem& p, cudaStream_t stream)
     a.keep_gate = static_cast<unsigned short*>(p.keep_gate);
     a.keep_up = static_cast<unsigned short*>(p.keep_up);
     a.m = p.m; a.n = p.n; a.k = p.k;
-    a.n_pad = p.m >= 128 ? 128 : (p.m + 15) / 16 * 16;
-    const int groups = (p.m + 127) / 128;
+    a.n_pad = l.n_pad;
+    a.stages = l.stages; a.stage_bytes = l.stage_bytes; a.cols = l.cols;
+    a.split = l.split;
+    a.tiles = l.tiles;
     a.act = p.act;
     a.fp16 = p.fp16;
     a.status = ctx->status_dev;
-    const int tiles = (p.n + kRows - 1) / kRows;
-    const int steps = (p.k + kStepK - 1) / kStepK;
-    a.tiles = tiles;
-    // About two CTAs per SM.  More rows of x make the reduction the larger part: a CTA then takes at least 4 steps
-    // (64 x 4096 x 4096 mxfp4: 7.9 us with 4 CTAs to a tile, 8.7 with 8; 16 rows: 6.3 and 6.2).
-    int split = 2 * ctx->sm_count / (tiles * groups);
-    if (a.n_pad > 32 && split > steps / 4) split = steps / 4;
-    split = split < 1 ? 1 : (split > 8 ? 8 : split);
-    if (split > steps) split = steps;
-    a.split = split;
-    const int steps_cta = (steps + split - 1) / split;
-    a.stage_bytes = (G::kOffX + a.n_pad * kStepBytes + 1023) / 1024 * 1024;
-    // As many stages as half an SM's shared memory takes, fewer where their scales do not fit half its tensor
-    // memory; the whole SM where not even two would fit.
-    const int acc = G::kW * a.n_pad;
-    int room = kSmShared / 2 - 1024 - 2048;  // less alignment and static part
-    int stages = room / a.stage_bytes < (256 - acc) / G::kScaleCols ? room / a.stage_bytes : (256 - acc) / G::kScaleCols;
-    if (acc >= 256 || stages < 2) {
-        room = kSmShared - 1024 - 2048;
-        stages = room / a.stage_bytes < (512 - acc) / G::kScaleCols ? room / a.stage_bytes : (512 - acc) / G::kScaleCols;
-    }
-    if (stages > kMaxStages) stages = kMaxStages;
-    if (stages > steps_cta) stages = steps_cta;
-    a.stages = stages;
-    const int cols = acc + stages * G::kScaleCols;
-    a.cols = cols <= 128 ? 128 : (cols <= 256 ? 256 : 512);
-    int smem = 1024 + stages * a.stage_bytes;
-    const int partials = split > 1 ? 1024 + G::kW * a.n_pad * kRows * 4 : 0;
-    if (smem < partials) smem = partials;
-    const int share = a.cols * kSharedPerCol - 1024;
-    if (smem < share) smem = share;
 
     const uint64_t pitch = static_cast<uint64_t>(p.k) / 2;
     CUtensorMap tm_x, tm_w, tm_w_up, tm_sx, tm_sw, tm_sw_up;
@@ -384,15 +344,15 @@ int launch_cfg(DeviceCtx* ctx, const Fp4Problem& p, cudaStream_t stream)
     if (rc != INT4L_OK) return rc;
 
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(tiles * split * groups, 1, 1);
+    cfg.gridDim = dim3(l.tiles * l.split * l.groups, 1, 1);
     cfg.blockDim = dim3(kThreads, 1, 1);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = l.smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = split;
+    attr[1].val.clusterDim.x = l.split;
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
@@ -406,7 +366,7 @@ int launch_cfg(DeviceCtx* ctx, const Fp4Problem& p, cudaStream_t stream)
 template <bool kBlock16, bool kGated>
 bool set_attr()
 {
-    return cudaFuncSetAttribute(gemm_fp4_fewrows_kernel<kBlock16, kGated>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmShared - 2048) == cudaSuccess;
+    return cudaFuncSetAttribute(gemm_fp4_fewrows_kernel<kBlock16, kGated>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmShared / 2) == cudaSuccess;
 }
 
 }  // namespace
@@ -416,16 +376,7 @@ int setup_fp4_fewrows(DeviceCtx*)
     return set_attr<false, false>() && set_attr<false, true>() && set_attr<true, false>() && set_attr<true, true>() ? INT4L_OK : INT4L_ERR_CUDA;
 }
 
-// Up to 64 rows this kernel is the faster one everywhere (64 x 14336 x 4096: 11.5 us against 11.9; 1 x 4096 x 4096: 6.1
-// against 8.2), from there on only where the tiles of gemm_fp4.cu leave most SMs idle for a long k: 128 x 1024 x 8192
-// 8.9 us against 13.9, 256 x 1024 x 8192 10.1 against 14.8, but 128 x 1024 x 1024 7.1 against 5.2 and 256 x 4096 x 4096
-// 10.8 against 9.9.  A gated tile has twice the partial sums to exchange and does not profit.
-bool fp4_fewrows_preferred(const DeviceCtx* ctx, const Fp4Problem& p)
-{
-    if (p.m <= 64) return true;
-    const int tiles = (p.n + kRows - 1) / kRows * ((p.m + 127) / 128);
-    return !p.gated && p.m <= 256 && p.k > 6144 && tiles <= ctx->sm_count / 4;
-}
+bool fp4_fewrows_preferred(const DeviceCtx* ctx, const Fp4Problem& p) { return fewrows_preferred(p.m, p.n, p.k, p.gated, ctx->sm_count); }
 
 int launch_fp4_fewrows(DeviceCtx* ctx, const Fp4Problem& p, cudaStream_t stream)
 {

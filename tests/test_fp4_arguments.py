@@ -1,8 +1,12 @@
-"""CPU: arguments of the microscaled operators that contradict one another."""
+"""CPU: arguments of the microscaled operators that contradict one another, and how sizes choose the few-rows kernel's launch."""
+import os
+import subprocess
+
 import pytest
 import torch
 
 import int4linear_b200 as L
+from conftest import ROOT
 from int4linear_b200 import fp4
 
 
@@ -15,6 +19,14 @@ def test_quantize_refuses_a_format_that_is_not_its_outputs():
             with pytest.raises(ValueError):
                 fp4._wanted_format(other, out)
     assert fp4._wanted_format(None, None) == "mxfp4" and fp4._wanted_format("nvfp4", None) == "nvfp4"
+
+
+def test_few_rows_launches(tmp_path):
+    exe = str(tmp_path / "fewrows_plan_check")
+    subprocess.run(["g++", "-O1", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover=undefined", "-o", exe,
+                    os.path.join(ROOT, "tests", "fewrows_plan_check.cpp")], check=True)
+    out = subprocess.run([exe], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "FEWROWS_OK" in out.stdout, out.stdout + out.stderr
 
 
 @pytest.mark.gpu
