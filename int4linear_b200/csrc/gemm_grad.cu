@@ -37,11 +37,10 @@
 //
 // Measured: 4096 x 4096 x 8192 nvfp4 360 us (1.53 PFLOP/s, tensor pipe 91 % busy at the 1.5 GHz the power limit leaves), gated
 // 4096 x 14336 x 4096 mxfp4 1.36 ms, of which the preparation takes 0.14 (it writes 0.7 GB).
-#include <cmath>
-
 #include "epilogue.cuh"
 #include "fp4_expand.cuh"
 #include "gate.cuh"
+#include "grad_plan.cuh"
 #include "grad_schedule.cuh"
 #include "ptx.cuh"
 
@@ -177,7 +176,7 @@ backward_prepare_kernel(const __grid_constant__ PrepArgs a)
 
 // ---------------------------------------------------------------- products
 
-constexpr int kBM = 128, kBN = 256, kStepK = 64;
+constexpr int kBM = 128;
 constexpr int kStage = 2 * 128 * 128;          // A and B tile of one CTA, 16 KB each
 constexpr int kChunk = kStepK * 128;           // a box: 64 columns x 64 rows
 constexpr int kStoreStage = 4096;              // per warp and buffer
@@ -199,14 +198,6 @@ struct Geo {
     static_assert(kSmemBytes <= 232448, "shared memory budget");
 };
 
-// One kind of tile: dx (its A operand is K-major), or a weight gradient (`matrices` of them, A MN-major).  A contraction
-// is `segments` runs of `seg_steps` steps, each over operands of its own, cut into `parts`.
-struct Kind {
-    int weight, matrices;
-    int rows, cols;         // of one result
-    int tiles_m, tiles_n;   // of one result
-    int segments, seg_steps, parts;
-};
 struct GradArgs {
     Kind kind[2];           // the one with the longer contraction first; kind[1] may have no tiles
     Deal deal;
@@ -595,72 +586,6 @@ sum_parts_kernel(const __grid_constant__ SumArgs a)
     }
     const float alpha = result_scale(j.num, j.den);
     *reinterpret_cast<uint2*>(j.out + at) = make_uint2(pack16<false>(sum.x * alpha, sum.y * alpha), pack16<false>(sum.z * alpha, sum.w * alpha));
-}
-
-// -------------------------------------------------------------------- plan
-
-// Everything that follows from the sizes alone: kinds, parts, and the workspace's pieces, each on a 256-byte boundary.
-struct Plan {
-    Kind dx, dw;
-    bool fine = false;
-    bool unpack = false;  // the products expand w and x themselves
-    long long tiles_dx = 0, tiles_dw = 0;
-    long long d[4] = {}, w[2] = {}, x = 0, partial[3] = {}, bytes = 0, ld = 0;
-};
-constexpr int kPlanWorkers = 74;  // CTA pairs of a B200
-constexpr int kTileSteps = 6;     // a tile's epilogue, in steps: it runs beside the next tile's steps, and is longer than few of them
-constexpr int kMinPart = 8;       // steps of a part: less would be the time of a tile's start and end
-constexpr int kMaxParts = 74;
-constexpr int kMinSaving = 24;    // steps (0.28 us each) that pay for the partial sums' way and the third launch
-
-Plan plan(long long m, long long n, long long k, bool gated, bool want_dx, bool want_dw)
-{
-    Plan p;
-    const int matrices = gated ? 2 : 1;
-    const int steps_n = static_cast<int>((n + kStepK - 1) / kStepK), steps_m = static_cast<int>((m + kStepK - 1) / kStepK);
-    const int tn = static_cast<int>((k + kBN - 1) / kBN);
-    p.dx = Kind{0, 1, static_cast<int>(m), static_cast<int>(k), static_cast<int>((m + 255) / 256), tn, matrices, steps_n, 1};
-    p.dw = Kind{1, matrices, static_cast<int>(n), static_cast<int>(k), static_cast<int>((n + 255) / 256), tn, 1, steps_m, 1};
-    // What is decided here does not depend on which gradients are wanted, so their bits do not either.
-    const double tiles_dx = static_cast<double>(p.dx.tiles_m) * tn, tiles_dw = static_cast<double>(matrices) * p.dw.tiles_m * tn;
-    const double load = (tiles_dx * matrices * steps_n + tiles_dw * steps_m) / kPlanWorkers;  // steps of a worker
-    // Expanded operands go to memory and come back: four times their bytes, twice, which few tokens do not repay, and
-    // it is a launch of its own.  The in-kernel expansion holds the products below 1.4 PFLOP/s.  Measured, in-kernel
-    // against expanded: mxfp4 64 x 8192 x 4096 49 us and 66, 256 rows 60 and 69, 512 rows 78 and 85, gated 512 rows 152
-    // and 158, 128 x 1024 x 1024 16 and 24; nvfp4 1024 rows 109 and 111; 4096 x 4096 x 8192 403 and 351.
-    p.unpack = m <= 512 || load <= 24.0;
-    // Two terms for dg and du where twice the steps are a few microseconds, or where there are so few values of them
-    // that the time goes into the weights.
-    p.fine = gated && (2.0 * load <= 24.0 || m * n <= 65536);
-    if (p.fine) {
-        p.dx.segments *= 2;
-        p.dw.segments *= 2;
-    }
-    auto cut = [&](Kind& kind, double tiles) {
-        // The time of the busiest worker, in steps, if only this kind existed; a part costs about kTileSteps besides.
-        const int steps = kind.segments * kind.seg_steps;
-        if (tiles >= 4.0 * kPlanWorkers) return;
-        double best = std::ceil(tiles / kPlanWorkers) * (steps + kTileSteps) - kMinSaving;
-        for (int parts = 2; parts <= kMaxParts && steps / parts >= kMinPart; ++parts) {
-            const double time = std::ceil(tiles * parts / kPlanWorkers) * ((steps + parts - 1) / parts + kTileSteps);
-            if (time < best) { best = time; kind.parts = parts; }
-        }
-    };
-    cut(p.dx, tiles_dx);
-    cut(p.dw, tiles_dw);
-    p.tiles_dx = want_dx ? static_cast<long long>(tiles_dx) * p.dx.parts : 0;
-    p.tiles_dw = want_dw ? static_cast<long long>(tiles_dw) * p.dw.parts : 0;
-
-    p.ld = (n + 7) / 8 * 8;
-    auto piece = [&](long long bytes) { const long long at = p.bytes; p.bytes += (bytes + 255) / 256 * 256; return at; };
-    if (gated || n % 8 != 0) p.d[0] = piece(m * p.ld * 2);  // (else dy is read as it is)
-    if (gated) p.d[1] = piece(m * p.ld * 2);
-    if (p.fine) { p.d[2] = piece(m * p.ld * 2); p.d[3] = piece(m * p.ld * 2); }
-    if (want_dx && !p.unpack) { p.w[0] = piece(n * k * 2); if (gated) p.w[1] = piece(n * k * 2); }
-    if (want_dw && !p.unpack) p.x = piece(m * k * 2);
-    if (want_dx && p.dx.parts > 1) p.partial[0] = piece(p.dx.parts * m * k * 4);
-    if (want_dw && p.dw.parts > 1) for (int i = 0; i < matrices; ++i) p.partial[1 + i] = piece(p.dw.parts * n * k * 4);
-    return p;
 }
 
 // The launch may begin while the one before it in the stream ends; the kernels wait before they touch memory.
