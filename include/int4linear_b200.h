@@ -245,6 +245,10 @@ int int4_linear_unpack_i32(const void* src_d, int* dst_d, int rows, int cols, vo
 #define INT4L_ACT_GELU      1  /* g times the normal distribution function of g      */
 #define INT4L_ACT_GELU_TANH 2  /* its tanh form                                      */
 
+/* Bits of the gate gradients of a gated backward pass, see below. */
+#define INT4L_GRAD_ONE_TERM  (1 << 8)
+#define INT4L_GRAD_TWO_TERMS (1 << 9)
+
 typedef struct int4_linear_fp4_matrix {
     const void* codes;
     const void* scales;
@@ -285,9 +289,13 @@ int int4_linear_fp4_gated_launch_async(const int4_linear_fp4_matrix* x, const in
  * aligned device memory of at least int4_linear_fp4_grad_workspace_bytes(...) bytes (0: none), free again when the
  * work on the stream is done; calls that can run at the same time need one each.
  *   linear  dx = dy w            dw = dy^T x                     (dy: m x n)
- *   gated   dg = dh up act'(gate), du = dh act(gate), rounded to bf16 (small problems: to twice its bits);
+ *   gated   dg = dh up act'(gate), du = dh act(gate);
  *           dx = dg w_gate + du w_up     dw_gate = dg^T x     dw_up = du^T x
- * gate_d and up_d are what the forward pass kept. */
+ * gate_d and up_d are what the forward pass kept, as bf16 (products kept as fp16 are not taken).
+ * dg and du are rounded to bf16, or carried as two bf16 terms (16 bits: the result's own rounding is then the only one that
+ * counts) in products of twice the length.  Without a flag the sizes decide: two terms where that takes a few
+ * microseconds at most, or where m n <= 65536.  INT4L_GRAD_ONE_TERM or INT4L_GRAD_TWO_TERMS, added to
+ * `activation` and, for the workspace, to `gated`, decides it for every size. */
 long long int4_linear_fp4_grad_workspace_bytes(int m, int n, int k, int gated, int want_dx, int want_dw);
 int int4_linear_fp4_grad_async(const void* dy_d, const int4_linear_fp4_matrix* x, const int4_linear_fp4_matrix* w,
                                void* dx_d, void* dw_d, void* workspace_d, long long workspace_bytes, void* stream);

@@ -45,6 +45,14 @@ int take_operands(const int4_linear_fp4_matrix* x, const int4_linear_fp4_matrix*
 
 bool bad_act(int act) { return act != INT4L_ACT_SILU && act != INT4L_ACT_GELU && act != INT4L_ACT_GELU_TANH; }
 
+// Takes INT4L_GRAD_*_TERM(S) out of a value: 1, 2, 0 for neither, -1 for both.
+int take_terms(int* value)
+{
+    const int flags = *value & (INT4L_GRAD_ONE_TERM | INT4L_GRAD_TWO_TERMS);
+    *value &= ~flags;
+    return flags == 0 ? 0 : flags == INT4L_GRAD_ONE_TERM ? 1 : flags == INT4L_GRAD_TWO_TERMS ? 2 : -1;
+}
+
 int launch_product(DeviceCtx* ctx, const Fp4Problem& p, cudaStream_t stream)
 {
     return fp4_fewrows_preferred(ctx, p) ? launch_fp4_fewrows(ctx, p, stream) : launch_fp4_gemm(ctx, p, stream);
@@ -56,7 +64,7 @@ int run_backward(Fp4Backward& b, void* workspace_d, long long workspace_bytes, v
     const Fp4Problem& p = b.forward;
     if (!b.dx && !b.dw) return INT4L_ERR_INVALID_ARG;
     if (misaligned(b.dx, 16) || misaligned(b.dw, 16) || misaligned(b.dw_up, 16) || misaligned(workspace_d, 256)) return INT4L_ERR_MISALIGNED;
-    const long long need = fp4_backward_workspace(p.m, p.n, p.k, p.gated, b.dx != nullptr, b.dw != nullptr);
+    const long long need = fp4_backward_workspace(p.m, p.n, p.k, p.gated, b.dx != nullptr, b.dw != nullptr, b.terms);
     if (need > 0 && (!workspace_d || workspace_bytes < need)) return INT4L_ERR_INVALID_ARG;
     int rc = INT4L_OK;
     DeviceCtx* ctx = current_ctx(&rc);
@@ -137,8 +145,9 @@ int int4_linear_fp4_gated_launch_async(const int4_linear_fp4_matrix* x, const in
 
 long long int4_linear_fp4_grad_workspace_bytes(int m, int n, int k, int gated, int want_dx, int want_dw)
 {
-    if (m <= 0 || n <= 0 || k <= 0) return -INT4L_ERR_INVALID_ARG;
-    return fp4_backward_workspace(m, n, k, gated != 0, want_dx != 0, want_dw != 0);
+    const int terms = take_terms(&gated);
+    if (m <= 0 || n <= 0 || k <= 0 || terms < 0) return -INT4L_ERR_INVALID_ARG;
+    return fp4_backward_workspace(m, n, k, gated != 0, want_dx != 0, want_dw != 0, terms);
 }
 
 int int4_linear_fp4_grad_async(const void* dy_d, const int4_linear_fp4_matrix* x, const int4_linear_fp4_matrix* w,
@@ -161,8 +170,9 @@ int int4_linear_fp4_gated_grad_async(const void* dh_d, const void* gate_d, const
                                      void* stream)
 {
     Fp4Backward b;
+    b.terms = take_terms(&activation);
     int rc = take_operands(x, w_gate, w_up, true, &b.forward);
-    if (rc == INT4L_OK && (!dh_d || !gate_d || !up_d || !dw_gate_d != !dw_up_d || bad_act(activation))) rc = INT4L_ERR_INVALID_ARG;
+    if (rc == INT4L_OK && (!dh_d || !gate_d || !up_d || !dw_gate_d != !dw_up_d || bad_act(activation) || b.terms < 0)) rc = INT4L_ERR_INVALID_ARG;
     if (rc == INT4L_OK && (misaligned(dh_d, 2) || misaligned(gate_d, 2) || misaligned(up_d, 2))) rc = INT4L_ERR_MISALIGNED;
     if (rc != INT4L_OK) return record_status(rc);
     b.forward.act = activation;

@@ -64,9 +64,10 @@ struct Fp4Backward {
     void* dx = nullptr;                   // m x k, or null
     void* dw = nullptr;                   // n x k, or null (gated: the gate's, and dw_up with it)
     void* dw_up = nullptr;
+    int terms = 0;                        // gated: bf16 terms of dg and du, 1 or 2, 0 by size
     uint8_t* workspace = nullptr;         // fp4_backward_workspace() bytes, 256-byte aligned
 };
-long long fp4_backward_workspace(long long m, long long n, long long k, bool gated, bool want_dx, bool want_dw);
+long long fp4_backward_workspace(long long m, long long n, long long k, bool gated, bool want_dx, bool want_dw, int terms);
 int setup_fp4_backward(DeviceCtx* ctx);
 int launch_fp4_backward(DeviceCtx* ctx, const Fp4Backward& b, cudaStream_t stream);
 int setup_fp4_gemm(DeviceCtx* ctx);

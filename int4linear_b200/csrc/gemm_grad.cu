@@ -8,8 +8,8 @@
 // share a scale, so the block-scaled instruction does not apply: the operands are expanded to bf16 first.  That
 // loses nothing (a code times its e8m0 or e4m3 scale has at most 6 significant bits).  Only dg and du are rounded, to
 // bf16 as the gradients of a bf16 network are: with the rounding of the result that is 1.4 times the error of one
-// rounding (2.4e-3 in the mean square against 1.7e-3).  Where it costs next to nothing (plan() says when) they are
-// carried as the sum of two bf16 values instead, 16 bits, as contractions of twice the length.
+// rounding (2.4e-3 in the mean square against 1.7e-3).  Where it costs next to nothing (plan() says when), or where the caller
+// asks for it, they are carried as the sum of two bf16 values instead, 16 bits, as contractions of twice the length.
 //
 // Up to three launches.  The first prepares: dg and du (or dy with a row pitch that TMA takes), and the expansions.  The second
 // is all products in one persistent kernel, a CTA pair per 256 x 256 tile (tcgen05.mma kind::f16, cta_group::2), two
@@ -603,9 +603,9 @@ bool unaligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) 
 
 }  // namespace
 
-long long fp4_backward_workspace(long long m, long long n, long long k, bool gated, bool want_dx, bool want_dw)
+long long fp4_backward_workspace(long long m, long long n, long long k, bool gated, bool want_dx, bool want_dw, int terms)
 {
-    return plan(m, n, k, gated, want_dx, want_dw).bytes;
+    return plan(m, n, k, gated, want_dx, want_dw, terms).bytes;
 }
 
 int setup_fp4_backward(DeviceCtx*)
@@ -621,7 +621,7 @@ int launch_fp4_backward(DeviceCtx* ctx, const Fp4Backward& b, cudaStream_t strea
 {
     using B = __nv_bfloat16;
     const Fp4Problem& p = b.forward;
-    const Plan l = plan(p.m, p.n, p.k, p.gated, b.dx != nullptr, b.dw != nullptr);
+    const Plan l = plan(p.m, p.n, p.k, p.gated, b.dx != nullptr, b.dw != nullptr, b.terms);
     uint8_t* ws = b.workspace;
     const bool direct = !p.gated && p.n % 8 == 0;  // dy as it is
     auto at = [&](long long piece) { return reinterpret_cast<B*>(ws + piece); };

@@ -32,7 +32,8 @@ constexpr int kMaxParts = 74;
 constexpr double kSumSteps = 12;       // the third launch, in steps (0.28 us each)
 constexpr double kStepBytes = 1.8e6;   // that pass through HBM in a step's time
 
-inline Plan plan(long long m, long long n, long long k, bool gated, bool want_dx, bool want_dw)
+// terms of dg and du: 1, 2, or 0 for the rule below.
+inline Plan plan(long long m, long long n, long long k, bool gated, bool want_dx, bool want_dw, int terms = 0)
 {
     Plan p;
     const int matrices = gated ? 2 : 1;
@@ -50,7 +51,7 @@ inline Plan plan(long long m, long long n, long long k, bool gated, bool want_dx
     p.unpack = m <= 512 || load <= 24.0;
     // Two terms for dg and du where twice the steps are a few microseconds, or where there are so few values of them
     // that the time goes into the weights.
-    p.fine = gated && (2.0 * load <= 24.0 || m * n <= 65536);
+    p.fine = gated && (terms == 2 || (terms == 0 && (2.0 * load <= 24.0 || m * n <= 65536)));
     if (p.fine) {
         p.dx.segments *= 2;
         p.dw.segments *= 2;

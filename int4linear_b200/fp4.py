@@ -311,7 +311,7 @@ def gated_linear_fp4(x: Fp4Matrix, w_gate: Fp4Matrix, w_up: Fp4Matrix, activatio
     """H = act(X @ Wg^T) * (X @ Wu^T), both products, the activation and the multiplication in one kernel.
 
     activation: "silu", "gelu" or "gelu_tanh".  Returns H, [m, n] bfloat16 (default) or float16; with `save`
-    (H, gate, up), the products rounded to the same type, as gated_linear_fp4_backward takes them."""
+    (H, gate, up), the products rounded to the same type; gated_linear_fp4_backward takes them in bfloat16."""
     import torch
     m, n = _check_operands(x, w_gate, w_up)
     dtype, t = _half(dtype, out)
@@ -331,6 +331,12 @@ def gated_linear_fp4(x: Fp4Matrix, w_gate: Fp4Matrix, w_up: Fp4Matrix, activatio
     return _run(body, x.device, stream, lambda: (*_parts(x, w_gate, w_up), out))
 
 
+def _terms_flag(terms: int | None) -> int:
+    if terms not in (None, 1, 2):
+        raise ValueError("terms is 1, 2 or None")
+    return {None: 0, 1: 1 << 8, 2: 1 << 9}[terms]
+
+
 def _check_grad(t, m: int, n: int, device, name: str):
     import torch
     if t.dtype != torch.bfloat16 or tuple(t.shape) != (m, n) or t.device != device:
@@ -339,7 +345,7 @@ def _check_grad(t, m: int, n: int, device, name: str):
 
 def _workspace(m, n, k, gated, want_x, want_w, device):
     import torch
-    need = _lib.load().int4_linear_fp4_grad_workspace_bytes(m, n, k, int(gated), int(want_x), int(want_w))
+    need = _lib.load().int4_linear_fp4_grad_workspace_bytes(m, n, k, gated, int(want_x), int(want_w))
     return torch.empty(max(need, 256), dtype=torch.uint8, device=device)
 
 
@@ -360,7 +366,7 @@ def linear_fp4_backward(grad_y, x: Fp4Matrix, w: Fp4Matrix, need=(True, True), s
             dy = grad_y.contiguous()
             if dy.data_ptr() % 16:
                 dy = dy.clone()
-            ws = _workspace(m, n, x.k, False, want_x, want_w, x.device)
+            ws = _workspace(m, n, x.k, 0, want_x, want_w, x.device)
             _check(_lib.load().int4_linear_fp4_grad_async(
                 dy.data_ptr(), x._p, w._p, dx.data_ptr() if want_x else None, dw.data_ptr() if want_w else None,
                 ws.data_ptr(), ws.numel(), handle), "int4_linear_fp4_grad_async")
@@ -370,18 +376,23 @@ def linear_fp4_backward(grad_y, x: Fp4Matrix, w: Fp4Matrix, need=(True, True), s
 
 
 def gated_linear_fp4_backward(grad_h, gate, up, x: Fp4Matrix, w_gate: Fp4Matrix, w_up: Fp4Matrix, activation: str = "silu",
-                              need=(True, True), stream=None):
+                              need=(True, True), stream=None, terms: int | None = None):
     """(dX, dWg, dWu) of gated_linear_fp4 in bfloat16, with respect to the values the operands stand for.
 
-    gate, up: the products kept by the forward pass, bfloat16 [m, n] like grad_h.
-    dG = dH up act'(gate) and dU = dH act(gate) are rounded to bfloat16 (small problems: to twice its bits); dX = dG Wg + dU Wu, dWg = dG^T X, dWu = dU^T X.
-    `need` = (input, weights) leaves gradients out (None in their place)."""
+    gate, up: the products kept by a forward pass in bfloat16, [m, n] like grad_h.
+    dG = dH up act'(gate), dU = dH act(gate); dX = dG Wg + dU Wu, dWg = dG^T X, dWu = dU^T X.
+    `need` = (input, weights) leaves gradients out (None in their place).
+    `terms`: 1 rounds dG and dU to bfloat16 (results then have 1.4 times the error of one rounding), 2 carries them as two
+    bfloat16 terms (one rounding) in products of twice the length (4096 x 14336 x 4096: 1.6 and 3.3 ms).  None lets the sizes decide: two terms where that
+    takes a few microseconds at most or m n <= 65536.  Give it where the bits of a token's gradient must not depend on the number
+    of tokens beside it in that way."""
     import torch
     m, n = _check_operands(x, w_gate, w_up)
     act = _check_act(activation)
     for t, name in ((grad_h, "grad_h"), (gate, "gate"), (up, "up")):
         _check_grad(t, m, n, x.device, name)
     want_x, want_w = bool(need[0]), bool(need[1])
+    flag = _terms_flag(terms)
 
     def body(handle):
         empty = m == 0 or n == 0
@@ -391,9 +402,9 @@ def gated_linear_fp4_backward(grad_h, gate, up, x: Fp4Matrix, w_gate: Fp4Matrix,
         dwu = new(n, x.k, dtype=torch.bfloat16, device=x.device) if want_w else None
         if not empty and (want_x or want_w):
             dh, g, u = grad_h.contiguous(), gate.contiguous(), up.contiguous()
-            ws = _workspace(m, n, x.k, True, want_x, want_w, x.device)
+            ws = _workspace(m, n, x.k, 1 | flag, want_x, want_w, x.device)
             _check(_lib.load().int4_linear_fp4_gated_grad_async(
-                dh.data_ptr(), g.data_ptr(), u.data_ptr(), x._p, w_gate._p, w_up._p, act, dx.data_ptr() if want_x else None,
+                dh.data_ptr(), g.data_ptr(), u.data_ptr(), x._p, w_gate._p, w_up._p, act | flag, dx.data_ptr() if want_x else None,
                 dwg.data_ptr() if want_w else None, dwu.data_ptr() if want_w else None, ws.data_ptr(), ws.numel(), handle),
                 "int4_linear_fp4_gated_grad_async")
         return dx, dwg, dwu

@@ -13,9 +13,9 @@ using namespace i4l;
 
 static int cases = 0;
 
-static bool workspace_ok(long long m, long long n, long long k, bool gated, bool want_dx, bool want_dw)
+static bool workspace_ok(long long m, long long n, long long k, bool gated, bool want_dx, bool want_dw, int terms)
 {
-    const Plan p = plan(m, n, k, gated, want_dx, want_dw);
+    const Plan p = plan(m, n, k, gated, want_dx, want_dw, terms);
     const long long matrices = gated ? 2 : 1;
     std::vector<std::pair<long long, long long>> pieces;  // begin, bytes
     if (gated || n % 8) for (int i = 0; i < matrices; ++i) pieces.push_back({p.d[i], m * p.ld * 2});
@@ -33,17 +33,18 @@ static bool workspace_ok(long long m, long long n, long long k, bool gated, bool
     return p.ld >= n && p.ld % 8 == 0 && end <= p.bytes && p.bytes < end + 256;
 }
 
-static int check(long long m, long long n, long long k, bool gated)
+static int check(long long m, long long n, long long k, bool gated, int terms)
 {
-    const Plan both = plan(m, n, k, gated, true, true);
+    const Plan both = plan(m, n, k, gated, true, true, terms);
+    if (terms && both.fine != (gated && terms == 2)) return 5;
     for (const Kind* kind : {&both.dx, &both.dw})
         if (kind->parts < 1 || kind->parts > kMaxParts || (kind->parts > 1 && kind->segments * kind->seg_steps / kind->parts < kMinPart)) return 1;
     for (int want = 1; want <= 3; ++want) {
         const bool dx = want & 1, dw = want & 2;
-        const Plan p = plan(m, n, k, gated, dx, dw);
+        const Plan p = plan(m, n, k, gated, dx, dw, terms);
         if (p.fine != both.fine || p.unpack != both.unpack || p.dx.parts != both.dx.parts || p.dw.parts != both.dw.parts) return 2;
         if (p.tiles_dx != (dx ? both.tiles_dx : 0) || p.tiles_dw != (dw ? both.tiles_dw : 0)) return 3;
-        if (!workspace_ok(m, n, k, gated, dx, dw)) return 4;
+        if (!workspace_ok(m, n, k, gated, dx, dw, terms)) return 4;
     }
     ++cases;
     return 0;
@@ -87,10 +88,11 @@ int main()
         for (long long n : rows)
             for (long long k : ks)
                 for (bool gated : {false, true})
-                    if (const int rc = check(m, n, k, gated)) {
-                        std::printf("FAIL %d: %s %lld x %lld x %lld\n", rc, gated ? "gated" : "linear", m, n, k);
-                        return 1;
-                    }
+                    for (int terms = 0; terms <= (gated ? 2 : 0); ++terms)
+                        if (const int rc = check(m, n, k, gated, terms)) {
+                            std::printf("FAIL %d: %s %lld x %lld x %lld, terms %d\n", rc, gated ? "gated" : "linear", m, n, k, terms);
+                            return 1;
+                        }
     std::printf("PLAN_OK %d\n", cases);
     return 0;
 }

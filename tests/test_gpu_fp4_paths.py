@@ -67,6 +67,30 @@ def test_gated_backward_in_one_term(cuda, fmt, m, n, k, act):
             assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m,n,k,act", [(300, 4100, 1056, "silu"), (1030, 4100, 1056, "gelu"), (515, 2731, 1056, "gelu_tanh"), (90, 200, 128, "silu")])
+def test_terms_decide_the_rounding(cuda, fmt, m, n, k, act):
+    """Two terms: an error of 2^-16 in dg and du, so what is left is the result's rounding.  One: another 2^-9 in the mean square.
+    Where the sizes decide, the bits are those of one or the other."""
+    x, wg, wu = (R.matrix(L, r, k, fmt, i, cuda, scale=0.25) for i, r in enumerate((m, n, n)))
+    gen = torch.Generator(device=cuda).manual_seed(m)
+    dh, gate, up = (torch.randn((m, n), generator=gen, device=cuda).to(torch.bfloat16) for _ in range(3))
+    g, u, d = gate.double(), up.double(), dh.double()
+    dg, du = d * u * R.act_slope(g, act), d * R.act(g, act)
+    xv, gv, uv = R.values(x), R.values(wg), R.values(wu)
+    want = (dg @ gv + du @ uv, dg.t() @ xv, du.t() @ xv)
+    one, two, auto = (L.gated_linear_fp4_backward(dh, gate, up, x, wg, wu, act, terms=t) for t in (1, 2, None))
+    for a, b, w in zip(one, two, want):
+        rounding = (w.to(torch.bfloat16).double() - w).norm()
+        assert (b.double() - w).norm() <= 1.05 * rounding < (a.double() - w).norm() <= 2 * rounding
+    for a, b in zip(auto, two if m * n <= 65536 else one):
+        assert torch.equal(a, b)
+    only_x = L.gated_linear_fp4_backward(dh, gate, up, x, wg, wu, act, need=(True, False), terms=2)[0]
+    only_w = L.gated_linear_fp4_backward(dh, gate, up, x, wg, wu, act, need=(False, True), terms=2)[1:]
+    for a, b in zip((only_x, *only_w), two):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("m,n", [(70, 264), (70, 131), (700, 1000)])
 def test_strided_gradients(cuda, m, n):
     x, wg, wu = (R.matrix(L, r, 96, "nvfp4", i, cuda) for i, r in enumerate((m, n, n)))
