@@ -286,7 +286,8 @@ int int4_linear_fp4_gated_launch_async(const int4_linear_fp4_matrix* x, const in
 
 /* Backward passes, bf16 gradients, with respect to the values the operands stand for.  dx_d (m x k) and
  * the weight gradients (n x k) may be left out with NULL, not all of them.  The workspace is 256-byte
- * aligned device memory of at least int4_linear_fp4_grad_workspace_bytes(...) bytes (0: none), free again when the
+ * aligned device memory of at least int4_linear_fp4_grad_workspace_bytes(...) bytes (0: none; minus a status code where
+ * the sizes are refused), free again when the
  * work on the stream is done; calls that can run at the same time need one each.
  *   linear  dx = dy w            dw = dy^T x                     (dy: m x n)
  *   gated   dg = dh up act'(gate), du = dh act(gate);

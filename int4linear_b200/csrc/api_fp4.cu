@@ -147,6 +147,7 @@ long long int4_linear_fp4_grad_workspace_bytes(int m, int n, int k, int gated, i
 {
     const int terms = take_terms(&gated);
     if (m <= 0 || n <= 0 || k <= 0 || terms < 0) return -INT4L_ERR_INVALID_ARG;
+    if (m > INT4L_FP4_MAX_EXTENT || n > INT4L_FP4_MAX_EXTENT || k > INT4L_FP4_MAX_EXTENT) return -INT4L_ERR_TOO_LARGE;
     return fp4_backward_workspace(m, n, k, gated != 0, want_dx != 0, want_dw != 0, terms);
 }
 

@@ -62,3 +62,12 @@ def test_terms_of_the_gate_gradients():
     for bad in (0, 3, "2"):
         with pytest.raises(ValueError):
             fp4._terms_flag(bad)
+
+
+def test_workspace_of_sizes_that_no_call_takes():
+    """Sizes beyond the operators' are refused before their bytes overflow."""
+    need = _lib.load().int4_linear_fp4_grad_workspace_bytes
+    for sizes in ((2 ** 31 - 1,) * 3, (2 ** 26 + 1, 8, 64), (8, 2 ** 26 + 1, 64), (8, 8, 2 ** 26 + 32)):
+        for gated in (0, 1):
+            assert need(*sizes, gated, 1, 1) == -7
+    assert need(2 ** 26, 2 ** 26, 2 ** 26, 1, 1, 1) > 2 ** 54
