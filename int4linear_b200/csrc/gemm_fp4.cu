@@ -30,8 +30,9 @@
 // thread of a converged warp issues them (with `if (lane == 0)` the step took 0.56 us instead of 0.36), with 32-bit
 // descriptor arithmetic (nvfp4 gated 4096 x 8192 x 2048: 63 -> 57 us).
 //
-// Measured: 8192 x 8192 x 16384 mxfp4 335 us (6.56 PFLOP/s), 8192^3 nvfp4 193 us (5.7), gated gelu 4096 x 14336 x 4096
-// nvfp4 180 us (5.35); at 8192^3 the tensor pipe is 82 % busy at 1.57 GHz, the clock that the power limit leaves.
+// Measured, a single call on an idle GPU and, under the power limit, call after call: 8192 x 8192 x 16384 mxfp4 334 and 421 us (6.6 and
+// 5.2 PFLOP/s), 8192^3 nvfp4 179 and 231 us, gated gelu 4096 x 14336 x 4096 nvfp4 174 and 215 us (262 and 257 with both
+// products kept); at 8192^3 the tensor pipe is 82 % busy at 1.57 GHz, the clock that the limit leaves.
 #include "epilogue.cuh"
 #include "fp4.cuh"
 #include "gate.cuh"

@@ -35,8 +35,9 @@
 // kind first to the workers that got one fewer, then round-robin (grad_schedule.cuh; gated 4096 x 14336 x 4096 on 74
 // pairs, in tile times of the weight gradients: 28 + 13 + 13 apart, 49 together, 48.4 the mean).
 //
-// Measured: 4096 x 4096 x 8192 nvfp4 360 us (1.53 PFLOP/s, tensor pipe 91 % busy at the 1.5 GHz the power limit leaves), gated
-// 4096 x 14336 x 4096 mxfp4 1.36 ms, of which the preparation takes 0.14 (it writes 0.7 GB).
+// Measured, a single call on an idle GPU and, under the power limit, call after call: 4096 x 4096 x 8192 nvfp4 352 and 430 us (1.56 and 1.28
+// PFLOP/s, tensor pipe 91 % busy at the 1.5 GHz the limit leaves), gated 4096 x 14336 x 4096 mxfp4 1.35 and 1.60 ms, of which
+// the preparation takes 0.14 (it writes 0.7 GB); dx alone 237 and 226 us, 1.02 and 0.93 ms.
 #include "epilogue.cuh"
 #include "fp4_expand.cuh"
 #include "gate.cuh"

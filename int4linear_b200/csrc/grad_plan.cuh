@@ -46,8 +46,10 @@ inline Plan plan(long long m, long long n, long long k, bool gated, bool want_dx
     const double load = (tiles_dx * matrices * steps_n + tiles_dw * steps_m) / kPlanWorkers;  // steps of a worker
     // Expanded operands go to memory and come back: four times their bytes, twice, which few tokens do not repay, and
     // it is a launch of its own.  The in-kernel expansion holds the products below 1.4 PFLOP/s.  Measured, in-kernel
-    // against expanded: mxfp4 64 x 8192 x 4096 49 us and 66, 256 rows 60 and 69, 512 rows 78 and 85, gated 512 rows 152
-    // and 158, 128 x 1024 x 1024 16 and 24; nvfp4 1024 rows 109 and 111; 4096 x 4096 x 8192 403 and 351.
+    // against expanded, back to back in a graph: mxfp4 64 x 8192 x 4096 45 us and 54 (dx alone 27 and 36), 256 rows 55 and 64, 512 rows
+    // 82 and 89, 1024 rows 131 and 127, gated 512 rows 164 and 177; nvfp4 1024 rows 129 and 132, 4096 x 4096 x 8192 444
+    // and 424.  A small layer gains by the launch it saves, called from a program (128 x 1024 x 1024 14.2 us and 16.4, 1021 rows
+    // 14.3 and 16.5), and loses as much in a graph, where launches are cheap; 600 x 3000 x 1024 19.8 and 20.7.
     p.unpack = m <= 512 || load <= 24.0;
     // Two terms for dg and du where twice the steps are a few microseconds, or where there are so few values of them
     // that the time goes into the weights.
