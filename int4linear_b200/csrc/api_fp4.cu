@@ -91,7 +91,7 @@ int int4_linear_fp4_quantize_async(const void* src_d, int src_type, long long sr
     if (rc == INT4L_OK && misaligned(src_d, element_bytes(src_type))) rc = INT4L_ERR_MISALIGNED;
     if (rc != INT4L_OK) return record_status(rc);
     DeviceCtx* ctx = current_ctx(&rc);
-    if (ctx) rc = launch_fp4_quantize(ctx, src_d, src_type, src_pitch, d, static_cast<cudaStream_t>(stream));
+    if (ctx) rc = launch_fp4_quantize(src_d, src_type, src_pitch, d, static_cast<cudaStream_t>(stream));
     return record_status(rc);
 }
 
@@ -103,7 +103,7 @@ int int4_linear_fp4_dequantize_async(const int4_linear_fp4_matrix* src, void* ds
     if (rc == INT4L_OK && misaligned(dst_d, 16)) rc = INT4L_ERR_MISALIGNED;
     if (rc != INT4L_OK) return record_status(rc);
     DeviceCtx* ctx = current_ctx(&rc);
-    if (ctx) rc = launch_fp4_dequantize(ctx, s, dst_d, dst_type, static_cast<cudaStream_t>(stream));
+    if (ctx) rc = launch_fp4_dequantize(s, dst_d, dst_type, static_cast<cudaStream_t>(stream));
     return record_status(rc);
 }
 

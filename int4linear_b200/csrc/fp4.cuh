@@ -38,6 +38,14 @@ __device__ __forceinline__ size_t fp4_scale_word(int row, int kt, int ktiles)
 }
 #endif
 
+// Map of a matrix's scales: one row per group of 128 matrix rows, 8-byte elements (a box has at most 256); a box takes the scale
+// tiles of one step of k (`step_bytes`) from `groups` groups.
+inline int fp4_scale_map(DeviceCtx* ctx, CUtensorMap* out, const Fp4& q, int step_bytes, int groups)
+{
+    const uint64_t row_bytes = static_cast<uint64_t>(fp4_ktiles(q.k, q.block16)) * kScaleTileBytes;
+    return encode_tensor_map_2d(ctx, out, q.scales, 8, row_bytes / 8, (q.rows + 127ll) / 128, row_bytes, step_bytes / 8, groups, false);
+}
+
 enum GateAct { kActSilu = INT4L_ACT_SILU, kActGelu = INT4L_ACT_GELU, kActGeluTanh = INT4L_ACT_GELU_TANH };
 
 // One product: y = x w^T (w_up null), or h = act(x w^T) * (x w_up^T).
@@ -53,8 +61,8 @@ struct Fp4Problem {
     int m = 0, n = 0, k = 0;
 };
 
-int launch_fp4_quantize(DeviceCtx* ctx, const void* src, int src_type, long long src_pitch, const Fp4& dst, cudaStream_t stream);
-int launch_fp4_dequantize(DeviceCtx* ctx, const Fp4& src, void* dst, int dst_type, cudaStream_t stream);
+int launch_fp4_quantize(const void* src, int src_type, long long src_pitch, const Fp4& dst, cudaStream_t stream);
+int launch_fp4_dequantize(const Fp4& src, void* dst, int dst_type, cudaStream_t stream);
 // Backward pass of a product or a gated product (gemm_grad.cu); x, w, w_up and m, n, k as in `forward`.
 struct Fp4Backward {
     Fp4Problem forward;

@@ -190,7 +190,7 @@ fp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restri
 }
 
 template <typename... P, typename... A>
-int launch_units(DeviceCtx* ctx, void (*kernel)(P...), long long rows, int k, int elems, cudaStream_t stream, A... args)
+int launch_units(void (*kernel)(P...), long long rows, int k, int elems, cudaStream_t stream, A... args)
 {
     const long long units = rows / kUnitRows * ((k + 32ll * elems - 1) / (32 * elems)), blocks = (units + kUnitThreads / 32 - 1) / (kUnitThreads / 32);
     if (blocks > 0x1FFFFFFF) return INT4L_ERR_TOO_LARGE;  // (units are counted in 32 bits; 4 T elements)
@@ -210,12 +210,12 @@ int launch_units(DeviceCtx* ctx, void (*kernel)(P...), long long rows, int k, in
 }
 
 template <int kType>
-int quantize_typed(DeviceCtx* ctx, const void* src, long long pitch, const Fp4& d, cudaStream_t stream)
+int quantize_typed(const void* src, long long pitch, const Fp4& d, cudaStream_t stream)
 {
     using T = typename Src<kType>::T;
     const long long rows = (d.rows + 127ll) / 128 * 128;
     auto launch = [&](auto kernel, int elems) {
-        return launch_units(ctx, kernel, rows, d.k, elems, stream, static_cast<const T*>(src), pitch, const_cast<uint8_t*>(d.codes),
+        return launch_units(kernel, rows, d.k, elems, stream, static_cast<const T*>(src), pitch, const_cast<uint8_t*>(d.codes),
                             const_cast<uint8_t*>(d.scales), d.tensor_scale, d.rows, d.k);
     };
     if (!d.block16) return launch(fp4_quantize_kernel<kType, false, 8>, 8);
@@ -226,30 +226,30 @@ int quantize_typed(DeviceCtx* ctx, const void* src, long long pitch, const Fp4& 
 }
 
 template <int kType>
-int dequantize_typed(DeviceCtx* ctx, const Fp4& s, void* dst, cudaStream_t stream)
+int dequantize_typed(const Fp4& s, void* dst, cudaStream_t stream)
 {
     using T = typename Src<kType>::T;
-    return launch_units(ctx, s.block16 ? fp4_dequantize_kernel<kType, true> : fp4_dequantize_kernel<kType, false>, (s.rows + 3ll) / 4 * 4, s.k, 8, stream,
+    return launch_units(s.block16 ? fp4_dequantize_kernel<kType, true> : fp4_dequantize_kernel<kType, false>, (s.rows + 3ll) / 4 * 4, s.k, 8, stream,
                         s.codes, s.scales, s.tensor_scale, static_cast<T*>(dst), s.rows, s.k);
 }
 
 }  // namespace
 
-int launch_fp4_quantize(DeviceCtx* ctx, const void* src, int src_type, long long src_pitch, const Fp4& dst, cudaStream_t stream)
+int launch_fp4_quantize(const void* src, int src_type, long long src_pitch, const Fp4& dst, cudaStream_t stream)
 {
     switch (src_type) {
-        case INT4L_TYPE_BF16: return quantize_typed<INT4L_TYPE_BF16>(ctx, src, src_pitch, dst, stream);
-        case INT4L_TYPE_F16: return quantize_typed<INT4L_TYPE_F16>(ctx, src, src_pitch, dst, stream);
-        default: return quantize_typed<INT4L_TYPE_F32>(ctx, src, src_pitch, dst, stream);
+        case INT4L_TYPE_BF16: return quantize_typed<INT4L_TYPE_BF16>(src, src_pitch, dst, stream);
+        case INT4L_TYPE_F16: return quantize_typed<INT4L_TYPE_F16>(src, src_pitch, dst, stream);
+        default: return quantize_typed<INT4L_TYPE_F32>(src, src_pitch, dst, stream);
     }
 }
 
-int launch_fp4_dequantize(DeviceCtx* ctx, const Fp4& src, void* dst, int dst_type, cudaStream_t stream)
+int launch_fp4_dequantize(const Fp4& src, void* dst, int dst_type, cudaStream_t stream)
 {
     switch (dst_type) {
-        case INT4L_TYPE_BF16: return dequantize_typed<INT4L_TYPE_BF16>(ctx, src, dst, stream);
-        case INT4L_TYPE_F16: return dequantize_typed<INT4L_TYPE_F16>(ctx, src, dst, stream);
-        default: return dequantize_typed<INT4L_TYPE_F32>(ctx, src, dst, stream);
+        case INT4L_TYPE_BF16: return dequantize_typed<INT4L_TYPE_BF16>(src, dst, stream);
+        case INT4L_TYPE_F16: return dequantize_typed<INT4L_TYPE_F16>(src, dst, stream);
+        default: return dequantize_typed<INT4L_TYPE_F32>(src, dst, stream);
     }
 }
 

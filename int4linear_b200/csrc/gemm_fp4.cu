@@ -322,14 +322,6 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
     }
 }
 
-// Map of a matrix's scales: one row per group of 128 matrix rows, 8-byte elements; `groups` rows per box.
-template <bool kBlock16>
-int scale_map(DeviceCtx* ctx, CUtensorMap* out, const Fp4& q, int groups)
-{
-    const uint64_t row_bytes = static_cast<uint64_t>(fp4_ktiles(q.k, kBlock16)) * kScaleTileBytes;
-    return encode_tensor_map_2d(ctx, out, q.scales, 8, row_bytes / 8, (q.rows + 127ll) / 128, row_bytes, Geo<kBlock16>::kScaleBytesA / 8, groups, false);
-}
-
 template <bool kBlock16, bool kGated, bool kHalf>
 int launch_cfg(DeviceCtx* ctx, const Fp4Problem& p, cudaStream_t stream)
 {
@@ -349,13 +341,13 @@ int launch_cfg(DeviceCtx* ctx, const Fp4Problem& p, cudaStream_t stream)
     CUtensorMap tm_x, tm_w, tm_w_up, tm_sx, tm_sw, tm_sw_up, tm_y, tm_g, tm_u;
     int rc = encode_tensor_map_2d(ctx, &tm_x, p.x.codes, 1, pitch, p.m, pitch, kStepBytes, kBM, true);
     if (rc == INT4L_OK) rc = encode_tensor_map_2d(ctx, &tm_w, p.w.codes, 1, pitch, p.n, pitch, kStepBytes, 128, true);
-    if (rc == INT4L_OK) rc = scale_map<kBlock16>(ctx, &tm_sx, p.x, 1);
-    if (rc == INT4L_OK) rc = scale_map<kBlock16>(ctx, &tm_sw, p.w, kGated ? 1 : 2);
+    if (rc == INT4L_OK) rc = fp4_scale_map(ctx, &tm_sx, p.x, Geo<kBlock16>::kScaleBytesA, 1);
+    if (rc == INT4L_OK) rc = fp4_scale_map(ctx, &tm_sw, p.w, Geo<kBlock16>::kScaleBytesA, kGated ? 1 : 2);
     tm_w_up = tm_w;
     tm_sw_up = tm_sw;
     if (rc == INT4L_OK && kGated) {
         rc = encode_tensor_map_2d(ctx, &tm_w_up, p.w_up.codes, 1, pitch, p.n, pitch, kStepBytes, 128, true);
-        if (rc == INT4L_OK) rc = scale_map<kBlock16>(ctx, &tm_sw_up, p.w_up, 1);
+        if (rc == INT4L_OK) rc = fp4_scale_map(ctx, &tm_sw_up, p.w_up, Geo<kBlock16>::kScaleBytesA, 1);
     }
     tm_y = tm_x;
     if (rc == INT4L_OK && a.tma_store) rc = encode_tensor_map_2d(ctx, &tm_y, p.y, 2, p.n, p.m, out_pitch, 64, 32, true);

@@ -303,13 +303,6 @@ gemm_fp4_fewrows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
     }
 }
 
-template <bool kBlock16>
-int scale_map(DeviceCtx* ctx, CUtensorMap* out, const Fp4& q)
-{
-    const uint64_t row_bytes = static_cast<uint64_t>(fp4_ktiles(q.k, kBlock16)) * kScaleTileBytes;
-    return encode_tensor_map_2d(ctx, out, q.scales, 8, row_bytes / 8, (q.rows + 127ll) / 128, row_bytes, Geo<kBlock16, false>::kScaleBytes / 8, 1, false);
-}
-
 template <bool kBlock16, bool kGated>
 int launch_cfg(DeviceCtx* ctx, const Fp4Problem& p, cudaStream_t stream)
 {
@@ -333,13 +326,13 @@ int launch_cfg(DeviceCtx* ctx, const Fp4Problem& p, cudaStream_t stream)
     CUtensorMap tm_x, tm_w, tm_w_up, tm_sx, tm_sw, tm_sw_up;
     int rc = encode_tensor_map_2d(ctx, &tm_x, p.x.codes, 1, pitch, p.m, pitch, kStepBytes, a.n_pad, true);
     if (rc == INT4L_OK) rc = encode_tensor_map_2d(ctx, &tm_w, p.w.codes, 1, pitch, p.n, pitch, kStepBytes, kRows, true);
-    if (rc == INT4L_OK) rc = scale_map<kBlock16>(ctx, &tm_sx, p.x);
-    if (rc == INT4L_OK) rc = scale_map<kBlock16>(ctx, &tm_sw, p.w);
+    if (rc == INT4L_OK) rc = fp4_scale_map(ctx, &tm_sx, p.x, Geo<kBlock16, kGated>::kScaleBytes, 1);
+    if (rc == INT4L_OK) rc = fp4_scale_map(ctx, &tm_sw, p.w, Geo<kBlock16, kGated>::kScaleBytes, 1);
     tm_w_up = tm_w;
     tm_sw_up = tm_sw;
     if (rc == INT4L_OK && kGated) {
         rc = encode_tensor_map_2d(ctx, &tm_w_up, p.w_up.codes, 1, pitch, p.n, pitch, kStepBytes, kRows, true);
-        if (rc == INT4L_OK) rc = scale_map<kBlock16>(ctx, &tm_sw_up, p.w_up);
+        if (rc == INT4L_OK) rc = fp4_scale_map(ctx, &tm_sw_up, p.w_up, Geo<kBlock16, kGated>::kScaleBytes, 1);
     }
     if (rc != INT4L_OK) return rc;
 
